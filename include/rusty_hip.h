@@ -309,6 +309,120 @@ int rusty_hip_attention_noalloc(const float *query, uintptr_t query_len, const f
                                 uintptr_t value_dim, uintptr_t key_stride, uintptr_t value_stride,
                                 uintptr_t slot_count, uintptr_t start_t, uintptr_t end_t, float scale, int use_sink);
 
+/* ===== Paged 4-bit KV cache (no reference counterpart) ======================
+ *
+ * The resident decoder holds one session's cache, so the reference keeps its
+ * multi-session server off it (src/metal.rs:375-390).  Here the sessions of a
+ * batch share one pool of pages per layer, with keys and values held as 4-bit
+ * codes in groups of 32 channels and one half-precision scale per group (the
+ * values d (c - 8) of GGUF's Q4_0): 4.5 bits per value.
+ *
+ * All pointers inside the structs are DEVICE memory of the library's device
+ * (device 0); the structs themselves are host memory and are read during the
+ * call.  The calls are asynchronous: they enqueue kernels on `stream` (a
+ * hipStream_t, NULL = the device's null stream), allocate nothing, keep nothing
+ * between calls, and may be captured into a HIP graph.  Calls on different
+ * streams may overlap as long as they do not share a workspace or rows they
+ * write.  They return 1 once enqueued and 0 (nothing enqueued) on a null
+ * pointer, a size or stride out of range, a buffer shorter than the call would
+ * touch, a misaligned pointer, a stream of another device, or a device error.
+ *
+ * What lies in device memory cannot be checked by the host; the kernels keep
+ * every access inside the buffers whatever it holds.  A page id outside
+ * [0, n_pages) or a position behind the page table's row stores nothing, reads
+ * nothing and is masked out of attention.  Rows that belong to no session (rows
+ * behind the last session's, or starts that do not ascend) are left as they
+ * were. */
+typedef struct {
+    uint8_t *k_pages, *v_pages; /* 16-byte aligned, rusty_hip_paged_kv_bytes each */
+    uintptr_t k_len, v_len;     /* bytes */
+    uint32_t n_pages;
+    uint32_t page_size;         /* tokens of a page, a multiple of 16, at most 65536 */
+    uint32_t n_kv_heads;
+    uint32_t head_dim, value_dim; /* multiples of 8, at most 256 */
+} RustyPagedKv;
+
+/* The rows of one call, ragged over the sessions: session s owns rows
+ * q_starts[s] .. q_starts[s + 1] - 1, which are its last ones, so row
+ * q_starts[s] + i has position kv_lens[s] - (q_starts[s + 1] - q_starts[s]) + i.
+ * Position p of session s lies in page page_table[s * table_stride + p /
+ * page_size].  A session may own no row. */
+typedef struct {
+    const int32_t *page_table;  /* [n_seqs][table_stride] */
+    const int32_t *kv_lens;     /* [n_seqs] tokens in the cache, this call's among them */
+    const int32_t *q_starts;    /* [n_seqs + 1] */
+    uintptr_t page_table_len, kv_lens_len, q_starts_len; /* bytes */
+    uint32_t n_seqs, table_stride;
+    uint32_t n_rows;            /* rows of the call's row buffers, the last session's end or more */
+    uint32_t max_q_len;         /* most rows of a session: later rows of one are not attended for */
+    uint32_t max_kv_len;        /* about the longest session; sizes the work's split, any value is correct */
+} RustyPagedBatch;
+
+/* Row buffers: row r of x starts at x + r * x_stride elements (float, or bf16
+ * with dtype = 1); rows are [heads][dim] without gaps.  Bases are aligned to
+ * four elements, strides are multiples of four.  x_len: bytes from x that the
+ * call may touch. */
+typedef struct {
+    uint32_t dtype;             /* of all rows: 0 = f32, 1 = bf16 */
+    uint32_t n_heads;           /* query heads (0 without q) */
+    const void *q, *k, *v;      /* q may be null: keys and values only */
+    void *q_out;                /* rotated queries, may be q itself */
+    uintptr_t q_len, k_len, v_len, q_out_len;
+    int64_t q_stride, k_stride, v_stride, q_out_stride;
+    const float *cos_t, *sin_t; /* [max_pos][rot_dim / 2], 16-byte aligned */
+    uintptr_t table_len;        /* bytes of each */
+    uint32_t max_pos;           /* rows at or behind it are left out whole */
+    uint32_t rot_dim;           /* rotated channels of a head, a multiple of 16, 0 = none */
+    uint32_t neox;              /* pairs (i, i + rot_dim / 2) instead of (2 i, 2 i + 1) */
+} RustyPagedAppend;
+
+typedef struct {
+    uint32_t dtype;
+    void *k, *v;                /* [n_kv_heads][head_dim] / [value_dim] rows; one may be null */
+    uintptr_t k_len, v_len;
+    int64_t k_stride, v_stride;
+} RustyPagedRead;
+
+typedef struct {
+    uint32_t dtype;
+    uint32_t n_heads;           /* a multiple of n_kv_heads */
+    const void *q;
+    void *out;                  /* [n_heads][value_dim] rows */
+    uintptr_t q_len, out_len;
+    int64_t q_stride, out_stride;
+    const float *sinks;         /* [n_heads] or null */
+    uintptr_t sinks_len;
+    float scale;
+    uint32_t window;            /* row at p sees (p - window, p]; 0 = all of [0, p] */
+    void *workspace;            /* rusty_hip_paged_attention_workspace bytes, 16-byte aligned; may be null if that is 0 */
+    uintptr_t workspace_len;
+} RustyPagedAttention;
+
+/* Bytes of the K and of the V pages of a pool; 0 for sizes that are not taken. */
+uint64_t rusty_hip_paged_kv_bytes(uint32_t n_pages, uint32_t page_size, uint32_t n_kv_heads, uint32_t head_dim,
+                                  uint32_t value_dim);
+/* Rotates the rows' queries and keys to their positions (apply_rope_qk /
+ * apply_rope_qk_neox, src/model.rs:5562-5647, with the caller's cos/sin table),
+ * stores the queries to q_out and quantizes keys and values into their pages.
+ * Rows of one call that fall on one position of a page (two sessions sharing a
+ * page they both write) leave either's bytes there. */
+int rusty_hip_paged_append(const RustyPagedKv *kv, const RustyPagedBatch *batch, const RustyPagedAppend *rows,
+                           void *stream);
+/* The rows' stored keys and values as numbers: what rusty_hip_resident_kv_read
+ * is to the resident decoder's cache. */
+int rusty_hip_paged_read(const RustyPagedKv *kv, const RustyPagedBatch *batch, const RustyPagedRead *rows,
+                         void *stream);
+/* Workspace bytes of rusty_hip_paged_attention for this batch's sizes (the
+ * pointers are not looked at); 0 if none is needed or the sizes are not taken. */
+uint64_t rusty_hip_paged_attention_workspace(const RustyPagedKv *kv, const RustyPagedBatch *batch, uint32_t n_heads);
+/* Softmax attention of the rows' queries over their session's cached positions,
+ * causal from each row's own position, with sliding window and per-head sinks
+ * (as rusty_hip_attention).  A row whose masks leave nothing is 0.  Sums,
+ * maxima and scores are f32; for f32 rows every product keeps at least 16 bits
+ * of its factors, for bf16 rows p is rounded to bf16. */
+int rusty_hip_paged_attention(const RustyPagedKv *kv, const RustyPagedBatch *batch, const RustyPagedAttention *rows,
+                              void *stream);
+
 /* ===== GGUF on-disk path (src/gguf.rs; src/model.rs:40-120, 3573-3860,
  * 5180-5420) ============================================================== */
 

@@ -12,6 +12,7 @@
 #include "gemm_mfma.hip"
 #include "prefill.hip"
 #include "prefill_moe.hip"
+#include "paged_attention.hip"
 #include "gguf.hpp"
 
 #include <hip/hip_ext.h>
@@ -4377,6 +4378,305 @@ int rusty_hip_resident_load_gguf(const char *path, uint32_t max_len) {
         if (debug_on()) fprintf(stderr, "[rusty_hip] resident_load_gguf_impl: exception\n");
         return 0;
     }
+}
+
+}  // extern "C"
+
+// ---- paged 4-bit KV cache -------------------------------------------------------
+namespace rh {
+
+// Bytes a call touches of n rows of `width` elements at `stride`, or -1.
+static int64_t rows_bytes(uint32_t n, int64_t stride, int64_t width, int item) {
+    if (stride < 0 || stride > (1ll << 40) || stride % 4 || (n > 1 && stride < width)) return -1;
+    return n ? ((int64_t)(n - 1) * stride + width) * item : 0;
+}
+static bool rows_ok(const void *p, uintptr_t len, uint32_t n, int64_t stride, int64_t width, int item) {
+    const int64_t need = rows_bytes(n, stride, width, item);
+    return p && need >= 0 && (uint64_t)need <= len && (uintptr_t)p % (4 * item) == 0;
+}
+
+static int paged_groups(uint32_t hd, uint32_t vd) {
+    const uint32_t d = hd > vd ? hd : vd;
+    return d <= 64 ? 2 : d <= 128 ? 4 : 8;
+}
+static uint64_t paged_bytes(uint32_t n_pages, uint32_t ps, uint32_t n_kv, uint32_t hd, uint32_t vd) {
+    if (n_pages == 0 || n_pages > 0x7FFFFFFFu || ps == 0 || ps % 16 || ps > 65536 || n_kv == 0 || n_kv > 4096 ||
+        hd == 0 || hd % 8 || hd > 256 || vd == 0 || vd % 8 || vd > 256)
+        return 0;
+    const uint64_t block = (uint64_t)ps * 18 * paged_groups(hd, vd), blocks = (uint64_t)n_pages * n_kv;
+    return blocks > (1ull << 46) / block ? 0 : blocks * block;  // 64 TB: above any memory, below any wrap
+}
+
+// The sizes of a call's cache and batch, and their buffers unless sizes_only.
+static bool paged_dev(const RustyPagedKv *kv, const RustyPagedBatch *b, PagedDev *P, bool sizes_only) {
+    if (!kv || !b) return false;
+    const uint64_t need = paged_bytes(kv->n_pages, kv->page_size, kv->n_kv_heads, kv->head_dim, kv->value_dim);
+    const uint32_t most = 1u << 24;  // rows, sessions and pages of a session
+    if (!need || b->n_seqs == 0 || b->n_seqs > most || b->table_stride == 0 || b->table_stride > most ||
+        b->n_rows == 0 || b->n_rows > most || b->max_q_len == 0)
+        return false;
+    if (!sizes_only &&
+        (!kv->k_pages || !kv->v_pages || kv->k_len < need || kv->v_len < need || (uintptr_t)kv->k_pages % 16 ||
+         (uintptr_t)kv->v_pages % 16 || !b->page_table || !b->kv_lens || !b->q_starts ||
+         b->page_table_len < (uint64_t)b->n_seqs * b->table_stride * 4 || b->kv_lens_len < (uint64_t)b->n_seqs * 4 ||
+         b->q_starts_len < ((uint64_t)b->n_seqs + 1) * 4 ||
+         ((uintptr_t)b->page_table | (uintptr_t)b->kv_lens | (uintptr_t)b->q_starts) % 4))
+        return false;
+    P->k = kv->k_pages;
+    P->v = kv->v_pages;
+    P->table = b->page_table;
+    P->kv_lens = b->kv_lens;
+    P->q_starts = b->q_starts;
+    P->n_pages = (int)kv->n_pages;
+    P->ps = (int)kv->page_size;
+    P->n_kv = (int)kv->n_kv_heads;
+    P->hd = (int)kv->head_dim;
+    P->vd = (int)kv->value_dim;
+    P->n_seqs = (int)b->n_seqs;
+    P->stride = (int)b->table_stride;
+    P->n_tokens = (int)b->n_rows;
+    P->block = (int64_t)kv->page_size * 18 * paged_groups(kv->head_dim, kv->value_dim);
+    return true;
+}
+
+// Launches run on the library's device, whichever is current in the caller's
+// thread; a stream of another device is refused.
+struct PagedDevice {
+    int before = -1;
+    bool ok = false;
+    explicit PagedDevice(hipStream_t s) {
+        {
+            std::lock_guard<std::mutex> lk(g.mu);
+            if (hipGetDevice(&before) != hipSuccess) before = -1;
+            ok = init_locked();
+        }
+        int now = -1;
+        if (ok && (hipGetDevice(&now) != hipSuccess || now != g.dev)) ok = hipSetDevice(g.dev) == hipSuccess;
+        if (ok && s) {
+            hipDevice_t d = 0;
+            ok = hipStreamGetDevice(s, &d) == hipSuccess && (int)d == g.dev;
+        }
+    }
+    ~PagedDevice() {
+        int now = -1;
+        if (before >= 0 && (hipGetDevice(&now) != hipSuccess || now != before)) (void)hipSetDevice(before);
+    }
+};
+
+// How a call's attention is cut: rows per tile, tiles, and splits of a tile's
+// cached range.
+struct PagedPlan {
+    int R, tok_tile, by_seq, n_splits, split_steps;
+    int64_t tiles, heads_y;
+};
+static PagedPlan paged_plan(const PagedDev &P, uint32_t n_heads, uint32_t max_q, uint32_t max_kv) {
+    PagedPlan p;
+    const int kv_mul = (int)n_heads / P.n_kv, chunk = kv_mul < 16 ? kv_mul : 16;
+    const bool wide = P.hd > 128 || P.vd > 128;  // 4-row tiles there would not fit the registers
+    const int64_t rows = (int64_t)chunk * (max_q < 16 ? max_q : 16);
+    p.R = rows <= 4 && !wide ? 4 : rows <= 8 ? 8 : 16;
+    p.tok_tile = p.R / chunk;
+    p.by_seq = max_q <= (uint32_t)p.tok_tile;
+    p.tiles = p.by_seq ? P.n_seqs : P.n_tokens / p.tok_tile + (int64_t)P.n_seqs;
+    p.heads_y = (int64_t)P.n_kv * ((kv_mul + 15) / 16);
+    const int64_t steps = ((int64_t)max_kv + 15 + 63) / 64 + 1;
+    // a workgroup takes four steps at a time; enough of them for four per CU
+    int64_t splits = (4 * 256 + p.tiles * p.heads_y - 1) / (p.tiles * p.heads_y);
+    const int64_t most = (steps + 3) / 4;
+    if (splits > most) splits = most;
+    if (splits > 256) splits = 256;
+    if (splits < 1) splits = 1;
+    p.n_splits = (int)splits;
+    p.split_steps = (int)((steps + splits - 1) / splits);
+    return p;
+}
+static uint64_t paged_workspace(const PagedDev &P, const PagedPlan &p, uint32_t n_heads) {
+    if (p.n_splits <= 1) return 0;
+    return (uint64_t)p.n_splits * P.n_tokens * n_heads * (32 * paged_groups(P.hd, P.vd) + 2) * 4;
+}
+static bool paged_heads_ok(const PagedDev &P, uint32_t n_heads) {
+    return n_heads && n_heads <= 65536 && n_heads % P.n_kv == 0;
+}
+
+template <int G, bool F32>
+static void paged_attn_launch(const PagedDev &P, const PagedAttn &A, const PagedPlan &p, hipStream_t s) {
+    const dim3 grid((unsigned)p.tiles, (unsigned)p.heads_y, (unsigned)p.n_splits);
+    if (p.R == 16)
+        paged_attn_rows_kernel<G, 16, F32><<<grid, 256, 0, s>>>(P, A);
+    else if (p.R == 8)
+        paged_attn_rows_kernel<G, 8, F32><<<grid, 256, 0, s>>>(P, A);
+    else if constexpr (G != 8)
+        paged_attn_rows_kernel<G, 4, F32><<<grid, 256, 0, s>>>(P, A);
+    if (p.n_splits > 1) {
+        const int64_t rows = (int64_t)P.n_tokens * A.n_heads;
+        paged_attn_join_kernel<G, F32><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(P, A);
+    }
+}
+
+}  // namespace rh
+
+extern "C" {
+
+uint64_t rusty_hip_paged_kv_bytes(uint32_t n_pages, uint32_t page_size, uint32_t n_kv_heads, uint32_t head_dim,
+                                  uint32_t value_dim) {
+    return rh::paged_bytes(n_pages, page_size, n_kv_heads, head_dim, value_dim);
+}
+
+int rusty_hip_paged_append(const RustyPagedKv *kv, const RustyPagedBatch *batch, const RustyPagedAppend *rows,
+                           void *stream) {
+    using namespace rh;
+    PagedDev P;
+    if (!rows || !paged_dev(kv, batch, &P, false) || rows->dtype > 1) return 0;
+    const int item = rows->dtype ? 2 : 4;
+    const uint32_t n = batch->n_rows;
+    const int64_t kw = (int64_t)P.n_kv * P.hd, vw = (int64_t)P.n_kv * P.vd;
+    if (!rows_ok(rows->k, rows->k_len, n, rows->k_stride, kw, item) ||
+        !rows_ok(rows->v, rows->v_len, n, rows->v_stride, vw, item))
+        return 0;
+    if (rows->q) {
+        const int64_t qw = (int64_t)rows->n_heads * P.hd;
+        if (!paged_heads_ok(P, rows->n_heads) || !rows_ok(rows->q, rows->q_len, n, rows->q_stride, qw, item) ||
+            !rows_ok(rows->q_out, rows->q_out_len, n, rows->q_out_stride, qw, item))
+            return 0;
+    }
+    if (rows->max_pos == 0 || rows->max_pos > 0x7FFFFFFFu || rows->rot_dim % 16 || rows->rot_dim > kv->head_dim)
+        return 0;
+    if (rows->rot_dim && (!rows->cos_t || !rows->sin_t || ((uintptr_t)rows->cos_t | (uintptr_t)rows->sin_t) % 16 ||
+                          rows->table_len < (uint64_t)rows->max_pos * (rows->rot_dim / 2) * 4))
+        return 0;
+    PagedDevice dev((hipStream_t)stream);
+    if (!dev.ok) return 0;
+    const int G = paged_groups(P.hd, P.vd);
+    PagedAppend A;
+    A.q = rows->q;
+    A.k = rows->k;
+    A.v = rows->v;
+    A.q_out = rows->q_out;
+    A.q_stride = rows->q_stride;
+    A.k_stride = rows->k_stride;
+    A.v_stride = rows->v_stride;
+    A.qo_stride = rows->q_out_stride;
+    A.cos_t = rows->cos_t;
+    A.sin_t = rows->sin_t;
+    A.n_heads = rows->q ? (int)rows->n_heads : 0;
+    A.max_pos = (int)rows->max_pos;
+    A.rot = (int)rows->rot_dim;
+    A.neox = rows->neox ? 1 : 0;
+    const int per = 64 / (P.hd / 8);
+    A.q_segs = (A.n_heads + per - 1) / per;
+    A.kv_segs = (P.n_kv * 4 * G + 63) / 64;
+    const int64_t waves = (int64_t)n * (A.q_segs + 2 * A.kv_segs);
+    if ((waves + 3) / 4 > 0x7FFFFFFF) return 0;
+    const unsigned grid = (unsigned)((waves + 3) / 4);
+    hipStream_t s = (hipStream_t)stream;
+#define RH_PAGED_APPEND(GG)                                                 \
+    if (rows->dtype)                                                        \
+        paged_append_kernel<GG, uint16_t><<<grid, 256, 0, s>>>(P, A);       \
+    else                                                                    \
+        paged_append_kernel<GG, float><<<grid, 256, 0, s>>>(P, A)
+    if (G == 2) {
+        RH_PAGED_APPEND(2);
+    } else if (G == 4) {
+        RH_PAGED_APPEND(4);
+    } else {
+        RH_PAGED_APPEND(8);
+    }
+#undef RH_PAGED_APPEND
+    RH_LAUNCH_OK();
+    return 1;
+}
+
+int rusty_hip_paged_read(const RustyPagedKv *kv, const RustyPagedBatch *batch, const RustyPagedRead *rows,
+                         void *stream) {
+    using namespace rh;
+    PagedDev P;
+    if (!rows || !paged_dev(kv, batch, &P, false) || rows->dtype > 1 || (!rows->k && !rows->v)) return 0;
+    const int item = rows->dtype ? 2 : 4;
+    const uint32_t n = batch->n_rows;
+    if ((rows->k && !rows_ok(rows->k, rows->k_len, n, rows->k_stride, (int64_t)P.n_kv * P.hd, item)) ||
+        (rows->v && !rows_ok(rows->v, rows->v_len, n, rows->v_stride, (int64_t)P.n_kv * P.vd, item)))
+        return 0;
+    PagedDevice dev((hipStream_t)stream);
+    if (!dev.ok) return 0;
+    const int G = paged_groups(P.hd, P.vd);
+    PagedRead A;
+    A.k = rows->k;
+    A.v = rows->v;
+    A.k_stride = rows->k_stride;
+    A.v_stride = rows->v_stride;
+    A.kv_segs = (P.n_kv * 4 * G + 63) / 64;
+    const int64_t waves = (int64_t)n * 2 * A.kv_segs;
+    if ((waves + 3) / 4 > 0x7FFFFFFF) return 0;
+    const unsigned grid = (unsigned)((waves + 3) / 4);
+    hipStream_t s = (hipStream_t)stream;
+#define RH_PAGED_READ(GG)                                                 \
+    if (rows->dtype)                                                      \
+        paged_read_kernel<GG, uint16_t><<<grid, 256, 0, s>>>(P, A);       \
+    else                                                                  \
+        paged_read_kernel<GG, float><<<grid, 256, 0, s>>>(P, A)
+    if (G == 2) {
+        RH_PAGED_READ(2);
+    } else if (G == 4) {
+        RH_PAGED_READ(4);
+    } else {
+        RH_PAGED_READ(8);
+    }
+#undef RH_PAGED_READ
+    RH_LAUNCH_OK();
+    return 1;
+}
+
+uint64_t rusty_hip_paged_attention_workspace(const RustyPagedKv *kv, const RustyPagedBatch *batch, uint32_t n_heads) {
+    using namespace rh;
+    PagedDev P;
+    if (!paged_dev(kv, batch, &P, true) || !paged_heads_ok(P, n_heads)) return 0;
+    return paged_workspace(P, paged_plan(P, n_heads, batch->max_q_len, batch->max_kv_len), n_heads);
+}
+
+int rusty_hip_paged_attention(const RustyPagedKv *kv, const RustyPagedBatch *batch, const RustyPagedAttention *rows,
+                              void *stream) {
+    using namespace rh;
+    PagedDev P;
+    if (!rows || !paged_dev(kv, batch, &P, false) || rows->dtype > 1 || !paged_heads_ok(P, rows->n_heads)) return 0;
+    const int item = rows->dtype ? 2 : 4;
+    const uint32_t n = batch->n_rows;
+    if (!rows_ok(rows->q, rows->q_len, n, rows->q_stride, (int64_t)rows->n_heads * P.hd, item) ||
+        !rows_ok(rows->out, rows->out_len, n, rows->out_stride, (int64_t)rows->n_heads * P.vd, item) ||
+        (rows->sinks && ((uintptr_t)rows->sinks % 4 || rows->sinks_len < (uint64_t)rows->n_heads * 4)) ||
+        rows->window > 0x7FFFFFFFu || !(rows->scale == rows->scale))
+        return 0;
+    PagedDevice dev((hipStream_t)stream);
+    if (!dev.ok) return 0;
+    const PagedPlan p = paged_plan(P, rows->n_heads, batch->max_q_len, batch->max_kv_len);
+    const uint64_t need = paged_workspace(P, p, rows->n_heads);
+    if (need && (!rows->workspace || rows->workspace_len < need || (uintptr_t)rows->workspace % 16)) return 0;
+    if (p.tiles > 0x7FFFFFFF || p.heads_y > 65535 || ((int64_t)n * rows->n_heads + 3) / 4 > 0x7FFFFFFF) return 0;
+    PagedAttn A;
+    A.q = rows->q;
+    A.out = rows->out;
+    A.sinks = rows->sinks;
+    A.part = need ? (float *)rows->workspace : nullptr;
+    A.ml = need ? A.part + (int64_t)p.n_splits * P.n_tokens * rows->n_heads * 32 * paged_groups(P.hd, P.vd) : nullptr;
+    A.q_stride = rows->q_stride;
+    A.o_stride = rows->out_stride;
+    A.scale = rows->scale * 1.44269504f;
+    A.n_heads = (int)rows->n_heads;
+    A.kv_mul = (int)rows->n_heads / P.n_kv;
+    A.window = (int)rows->window;
+    A.tok_tile = p.tok_tile;
+    A.n_splits = p.n_splits;
+    A.split_steps = p.split_steps;
+    A.by_seq = p.by_seq;
+    hipStream_t s = (hipStream_t)stream;
+    const int G = paged_groups(P.hd, P.vd);
+    if (rows->dtype)
+        G == 2 ? paged_attn_launch<2, false>(P, A, p, s)
+               : G == 4 ? paged_attn_launch<4, false>(P, A, p, s) : paged_attn_launch<8, false>(P, A, p, s);
+    else
+        G == 2 ? paged_attn_launch<2, true>(P, A, p, s)
+               : G == 4 ? paged_attn_launch<4, true>(P, A, p, s) : paged_attn_launch<8, true>(P, A, p, s);
+    RH_LAUNCH_OK();
+    return 1;
 }
 
 }  // extern "C"

@@ -37,6 +37,8 @@ SYMBOLS = [
     "rusty_hip_resident_load_gguf", "rusty_hip_resident_enable_bf16", "rusty_hip_debug_stream_mark",
     "rusty_hip_debug_alloc_limit",
     "rusty_hip_set_expert_mfma", "rusty_hip_mxfp4_experts",
+    "rusty_hip_paged_kv_bytes", "rusty_hip_paged_append", "rusty_hip_paged_read",
+    "rusty_hip_paged_attention_workspace", "rusty_hip_paged_attention",
 ]
 
 
@@ -661,3 +663,198 @@ def mxfp4_experts_dev(w_ptr, row_stride, exp_stride, n_exp, rows, cols, x_ptr, l
     return lib.rusty_hip_mxfp4_experts(w_ptr, row_stride, exp_stride, n_exp, rows, cols, x_ptr, ldx,
                                        1 if x_per_pair else 0, top_k, sel_ptr, n_pairs, y_ptr, ldy,
                                        1 if mfma else 0) == 1
+
+
+# ---- paged 4-bit KV cache of many sessions ------------------------------------------
+class _PagedKv(C.Structure):
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("k_len", C.c_size_t), ("v_len", C.c_size_t),
+                ("n_pages", C.c_uint32), ("page_size", C.c_uint32), ("n_kv_heads", C.c_uint32),
+                ("head_dim", C.c_uint32), ("value_dim", C.c_uint32)]
+
+
+class _PagedBatch(C.Structure):
+    _fields_ = [("page_table", C.c_void_p), ("kv_lens", C.c_void_p), ("q_starts", C.c_void_p),
+                ("page_table_len", C.c_size_t), ("kv_lens_len", C.c_size_t), ("q_starts_len", C.c_size_t),
+                ("n_seqs", C.c_uint32), ("table_stride", C.c_uint32), ("n_rows", C.c_uint32),
+                ("max_q_len", C.c_uint32), ("max_kv_len", C.c_uint32)]
+
+
+class _PagedAppend(C.Structure):
+    _fields_ = [("dtype", C.c_uint32), ("n_heads", C.c_uint32), ("q", C.c_void_p), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("q_out", C.c_void_p), ("q_len", C.c_size_t), ("k_len", C.c_size_t),
+                ("v_len", C.c_size_t), ("q_out_len", C.c_size_t), ("q_stride", C.c_int64), ("k_stride", C.c_int64),
+                ("v_stride", C.c_int64), ("q_out_stride", C.c_int64), ("cos_t", C.c_void_p), ("sin_t", C.c_void_p),
+                ("table_len", C.c_size_t), ("max_pos", C.c_uint32), ("rot_dim", C.c_uint32), ("neox", C.c_uint32)]
+
+
+class _PagedRead(C.Structure):
+    _fields_ = [("dtype", C.c_uint32), ("k", C.c_void_p), ("v", C.c_void_p), ("k_len", C.c_size_t),
+                ("v_len", C.c_size_t), ("k_stride", C.c_int64), ("v_stride", C.c_int64)]
+
+
+class _PagedAttention(C.Structure):
+    _fields_ = [("dtype", C.c_uint32), ("n_heads", C.c_uint32), ("q", C.c_void_p), ("out", C.c_void_p),
+                ("q_len", C.c_size_t), ("out_len", C.c_size_t), ("q_stride", C.c_int64), ("out_stride", C.c_int64),
+                ("sinks", C.c_void_p), ("sinks_len", C.c_size_t), ("scale", C.c_float), ("window", C.c_uint32),
+                ("workspace", C.c_void_p), ("workspace_len", C.c_size_t)]
+
+
+_sig("rusty_hip_paged_kv_bytes", C.c_uint64, _u32, _u32, _u32, _u32, _u32)
+_sig("rusty_hip_paged_append", _i, _p, _p, _p, _p)
+_sig("rusty_hip_paged_read", _i, _p, _p, _p, _p)
+_sig("rusty_hip_paged_attention_workspace", C.c_uint64, _p, _p, _u32)
+_sig("rusty_hip_paged_attention", _i, _p, _p, _p, _p)
+
+
+def paged_kv_bytes(n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, value_dim: int | None = None) -> int:
+    """Bytes of the K pages, and of the V pages, of a pool (0: sizes that are not taken)."""
+    return lib.rusty_hip_paged_kv_bytes(n_pages, page_size, n_kv_heads, head_dim, value_dim or head_dim)
+
+
+def _dev_bytes(t, what, dtype):
+    """A contiguous device tensor's address and bytes."""
+    if str(t.dtype) != "torch." + dtype or not t.is_contiguous() or not t.is_cuda:
+        raise ValueError(f"{what}: a contiguous {dtype} tensor on the GPU is needed")
+    return t.data_ptr(), t.numel() * t.element_size()
+
+
+class PagedKv:
+    """One layer's pool of cache pages (RustyPagedKv) over two uint8 device
+    tensors of paged_kv_bytes each.  The tensors stay the caller's."""
+
+    def __init__(self, k_pages, v_pages, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
+                 value_dim: int | None = None):
+        self.n_kv_heads, self.head_dim, self.value_dim = n_kv_heads, head_dim, value_dim or head_dim
+        self.device = k_pages.device
+        k, k_len = _dev_bytes(k_pages, "k_pages", "uint8")
+        v, v_len = _dev_bytes(v_pages, "v_pages", "uint8")
+        need = paged_kv_bytes(n_pages, page_size, n_kv_heads, head_dim, self.value_dim)
+        if need == 0 or k_len < need or v_len < need or v_pages.device != self.device:
+            raise ValueError("PagedKv: sizes that are not taken, or pages shorter than paged_kv_bytes")
+        self._c = _PagedKv(k, v, k_len, v_len, n_pages, page_size, n_kv_heads, head_dim, self.value_dim)
+        self._ref = C.addressof(self._c)
+        self._keep = (k_pages, v_pages)
+
+
+class PagedBatch:
+    """The rows of a call over the sessions (RustyPagedBatch): int32 device
+    tensors page_table [n_seqs][stride], kv_lens [n_seqs] and q_starts
+    [n_seqs + 1], whose contents may change between calls.  max_q_len: most
+    rows of one session; max_kv_len: about the longest session."""
+
+    def __init__(self, page_table, kv_lens, q_starts, max_q_len: int, max_kv_len: int):
+        n, stride = page_table.shape
+        if n == 0 or tuple(kv_lens.shape) != (n,) or tuple(q_starts.shape) != (n + 1,):
+            raise ValueError("PagedBatch: page_table [n][stride], kv_lens [n] and q_starts [n + 1] are needed")
+        self.device = page_table.device
+        if kv_lens.device != self.device or q_starts.device != self.device:
+            raise ValueError("PagedBatch: tensors of one device are needed")
+        t, t_len = _dev_bytes(page_table, "page_table", "int32")
+        l, l_len = _dev_bytes(kv_lens, "kv_lens", "int32")
+        q, q_len = _dev_bytes(q_starts, "q_starts", "int32")
+        self._c = _PagedBatch(t, l, q, t_len, l_len, q_len, n, stride, 0, max_q_len, max_kv_len)
+        self._ref = C.addressof(self._c)
+        self._keep = (page_table, kv_lens, q_starts)
+
+
+def _rows(kv, t, what, dtype, n, heads, dim):
+    """Address, bytes and row stride of a [rows][heads][dim] device tensor."""
+    if t.dtype != dtype or t.device != kv.device or tuple(t.shape) != (n, heads, dim):
+        raise ValueError(f"{what}: a {dtype} tensor [{n}][{heads}][{dim}] on {kv.device} is needed")
+    row, head, one = t.stride()
+    if (one != 1 and dim > 1) or (head != dim and heads > 1):
+        raise ValueError(f"{what}: rows without gaps are needed")
+    if n <= 1:
+        row = heads * dim
+    return t.data_ptr(), ((n - 1) * row + heads * dim) * t.element_size(), row
+
+
+_PAGED_DTYPE = {"torch.float32": 0, "torch.bfloat16": 1}
+
+
+def _paged_call(kv, batch, t, stream):
+    """dtype code and rows of the row tensor t, and the stream: the caller's, or
+    torch's current one on the cache's device."""
+    if batch.device != kv.device or kv.device.index not in (0, None):
+        raise ValueError("paged cache: one device, the library's (device 0), is needed")
+    code = _PAGED_DTYPE.get(str(t.dtype))
+    if code is None:
+        raise ValueError("paged cache: float32 or bfloat16 rows are needed")
+    if stream is None:
+        import torch
+        stream = torch.cuda.current_stream(kv.device).cuda_stream
+    batch._c.n_rows = t.shape[0]
+    return code, t.shape[0], stream
+
+
+def paged_append_dev(kv: PagedKv, batch: PagedBatch, k, v, cos, sin, q=None, q_out=None, neox: bool = False,
+                     stream: int | None = None) -> bool:
+    """rusty_hip_paged_append: rotates q (into q_out, which may be q) and k by
+    the f32 tables cos / sin [max_pos][rot_dim / 2], and quantizes k and v into
+    their pages.  Rows are [rows][heads][dim] device tensors, float32 or
+    bfloat16, of any row stride.  Asynchronous on `stream`."""
+    if not enabled():
+        return False
+    code, n, stream = _paged_call(kv, batch, k, stream)
+    t = k.dtype
+    a = _PagedAppend(dtype=code, neox=1 if neox else 0)
+    a.k, a.k_len, a.k_stride = _rows(kv, k, "k", t, n, kv.n_kv_heads, kv.head_dim)
+    a.v, a.v_len, a.v_stride = _rows(kv, v, "v", t, n, kv.n_kv_heads, kv.value_dim)
+    if q is not None:
+        heads = q.shape[1]
+        if q_out is None:
+            raise ValueError("paged_append_dev: q needs q_out (which may be q)")
+        a.n_heads = heads
+        a.q, a.q_len, a.q_stride = _rows(kv, q, "q", t, n, heads, kv.head_dim)
+        a.q_out, a.q_out_len, a.q_out_stride = _rows(kv, q_out, "q_out", t, n, heads, kv.head_dim)
+    if cos.shape != sin.shape or cos.device != kv.device or sin.device != kv.device:
+        raise ValueError("paged_append_dev: cos and sin [max_pos][rot_dim / 2] on the cache's device are needed")
+    a.cos_t, a.table_len = _dev_bytes(cos, "cos", "float32")
+    a.sin_t, _ = _dev_bytes(sin, "sin", "float32")
+    a.max_pos, a.rot_dim = cos.shape[0], 2 * cos.shape[1]
+    return lib.rusty_hip_paged_append(kv._ref, batch._ref, C.addressof(a), stream) == 1
+
+
+def paged_read_dev(kv: PagedKv, batch: PagedBatch, k_out=None, v_out=None, stream: int | None = None) -> bool:
+    """rusty_hip_paged_read: the rows' stored keys and values as numbers."""
+    if not enabled():
+        return False
+    first = k_out if k_out is not None else v_out
+    if first is None:
+        raise ValueError("paged_read_dev: k_out or v_out is needed")
+    code, n, stream = _paged_call(kv, batch, first, stream)
+    a = _PagedRead(dtype=code)
+    if k_out is not None:
+        a.k, a.k_len, a.k_stride = _rows(kv, k_out, "k_out", first.dtype, n, kv.n_kv_heads, kv.head_dim)
+    if v_out is not None:
+        a.v, a.v_len, a.v_stride = _rows(kv, v_out, "v_out", first.dtype, n, kv.n_kv_heads, kv.value_dim)
+    return lib.rusty_hip_paged_read(kv._ref, batch._ref, C.addressof(a), stream) == 1
+
+
+def paged_attention_workspace(kv: PagedKv, batch: PagedBatch, n_rows: int, n_heads: int) -> int:
+    """Workspace bytes of paged_attention_dev for n_rows rows of n_heads query heads."""
+    batch._c.n_rows = n_rows
+    return lib.rusty_hip_paged_attention_workspace(kv._ref, batch._ref, n_heads)
+
+
+def paged_attention_dev(kv: PagedKv, batch: PagedBatch, q, out, scale: float, workspace=None, sinks=None,
+                        window: int = 0, stream: int | None = None) -> bool:
+    """rusty_hip_paged_attention: attention of the rows' queries over their
+    session's pages.  workspace: a uint8 device tensor of
+    paged_attention_workspace bytes, used by one call at a time."""
+    if not enabled():
+        return False
+    code, n, stream = _paged_call(kv, batch, q, stream)
+    heads = q.shape[1]
+    a = _PagedAttention(dtype=code, n_heads=heads, scale=scale, window=window)
+    a.q, a.q_len, a.q_stride = _rows(kv, q, "q", q.dtype, n, heads, kv.head_dim)
+    a.out, a.out_len, a.out_stride = _rows(kv, out, "out", q.dtype, n, heads, kv.value_dim)
+    if sinks is not None:
+        if sinks.device != kv.device:
+            raise ValueError("paged_attention_dev: sinks on the cache's device are needed")
+        a.sinks, a.sinks_len = _dev_bytes(sinks, "sinks", "float32")
+    if workspace is not None:
+        if workspace.device != kv.device:
+            raise ValueError("paged_attention_dev: a workspace on the cache's device is needed")
+        a.workspace, a.workspace_len = _dev_bytes(workspace, "workspace", "uint8")
+    return lib.rusty_hip_paged_attention(kv._ref, batch._ref, C.addressof(a), stream) == 1
