@@ -39,8 +39,17 @@ struct PagedDev {
     const int32_t *kv_lens;   // [n_seqs]
     const int32_t *q_starts;  // [n_seqs + 1]
     int32_t n_pages, ps, n_kv, hd, vd, n_seqs, stride, n_tokens;
-    int64_t block;            // bytes of one (page, kv head)
+    uint32_t tile_mul, tile_shift;  // 16-token tile -> page, see page_of_tile
+    int64_t block;                  // bytes of one (page, kv head)
 };
+
+// n / d for n < 2^31 as (n * mul) >> shift: shift = 31 + ceil(log2 d), mul =
+// ceil(2^shift / d) <= 2^32 - 1 for d > 1, whose excess over 2^shift / d is below
+// 2^ceil(log2 d) / d, too little to reach the next quotient.  (An integer division
+// is about 25 instructions.)
+__host__ __device__ __forceinline__ int page_of_tile(const PagedDev &P, int tile) {
+    return P.tile_mul ? (int)((uint64_t)(uint32_t)tile * P.tile_mul >> P.tile_shift) : tile;
+}
 
 // Session of row t of the batch, wave-uniform: the last start at or below t, found
 // by 64 lanes at a time.  False for rows of no session: rows behind the last one,
@@ -70,13 +79,16 @@ __device__ __forceinline__ bool paged_row(const PagedDev &P, int t, int *seq, in
     return p >= 0;
 }
 
-// Page of a position, or -1: outside the table's row or the pool.
-__device__ __forceinline__ int paged_page(const PagedDev &P, int seq, int pos) {
-    const int i = pos / P.ps;
+// Page of a position, or -1: outside the table's row or the pool.  *off: token in it.
+__device__ __forceinline__ int paged_page(const PagedDev &P, int seq, int pos, int *off) {
+    const int i = page_of_tile(P, pos >> 4);
+    *off = pos - i * P.ps;
     if (i >= P.stride) return -1;
     const int page = P.table[(int64_t)seq * P.stride + i];
     return page >= 0 && page < P.n_pages ? page : -1;
 }
+// wave-uniform values into scalar registers
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // ---- element access: rows of f32 or bf16 ----------------------------------------
 __device__ __forceinline__ void row_load4(const float *p, float *x) {
@@ -199,9 +211,9 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedDev P, PagedAppe
     const bool is_v = seg >= A.kv_segs;
     const int u = (is_v ? seg - A.kv_segs : seg) * 64 + lane;
     const int head = u / (4 * G), g = (u % (4 * G)) >> 2, i = u & 3;
-    const int page = paged_page(P, seq, pos);
+    int off;
+    const int page = paged_page(P, seq, pos, &off);
     if (page < 0) return;
-    const int off = pos % P.ps;
     const bool on = head < P.n_kv;
     uint8_t *blk = (is_v ? P.v : P.k) + ((int64_t)page * P.n_kv + (on ? head : 0)) * P.block;
     float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -261,12 +273,12 @@ __global__ __launch_bounds__(256) void paged_read_kernel(PagedDev P, PagedRead A
     const int seg = (int)(w % (2 * A.kv_segs));
     int seq, pos;
     if (t >= P.n_tokens || !paged_row(P, t, &seq, &pos)) return;
-    const int page = paged_page(P, seq, pos);
+    int off;
+    const int page = paged_page(P, seq, pos, &off);
     if (page < 0) return;
     const bool is_v = seg >= A.kv_segs;
     const int u = (is_v ? seg - A.kv_segs : seg) * 64 + lane;
     const int head = u / (4 * G), g = (u % (4 * G)) >> 2, i = u & 3;
-    const int off = pos % P.ps;
     const bool on = head < P.n_kv;
     const uint8_t *blk = (is_v ? P.v : P.k) + ((int64_t)page * P.n_kv + (on ? head : 0)) * P.block;
     const float d = h2f(*(const uint16_t *)(blk + (int64_t)P.ps * (16 * G) + (off * G + g) * 2));

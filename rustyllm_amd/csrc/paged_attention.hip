@@ -20,16 +20,19 @@ struct PagedAttn {
     int64_t q_stride, o_stride;
     float scale;         // times log2(e)
     int32_t n_heads, kv_mul, window;
+    int32_t n_chunk;     // 16 query heads of a kv head at a time
+    int32_t inv16, inv;  // ceil(256 / heads) of a full chunk and of the last: row / heads for row < 16
     int32_t tok_tile;    // tokens of a row tile
     int32_t n_splits;    // most splits of a row tile's range
     int32_t split_steps; // 64-token steps of a split, more where n_splits would not cover the range
     int32_t by_seq;      // 1: tile x is session x (at most one tile each)
 };
 
-// Row tile x of the batch: its session, first token (of the session) and tokens.
-// Wave-uniform; 64 sessions per turn, each lane one session's tile count.
-__device__ __forceinline__ bool paged_tile(const PagedDev &P, const PagedAttn &A, int x, int *seq, int *tok,
-                                           int *n) {
+// Row tile x of the batch: its session, first token (of the session) and tokens, the
+// session's first row, and the first token's position.  Wave-uniform; 64 sessions
+// per turn, each lane one session's tile count.
+__device__ __forceinline__ bool paged_tile(const PagedDev &P, const PagedAttn &A, int x, int *seq, int *tok, int *n,
+                                           int *row0, int *pos0) {
     const int lane = threadIdx.x & 63;
     if (A.by_seq) {
         *seq = x;
@@ -61,9 +64,14 @@ __device__ __forceinline__ bool paged_tile(const PagedDev &P, const PagedAttn &A
         if (found < 0) return false;
         *seq = found;
     }
-    const int a = P.q_starts[*seq], b = P.q_starts[*seq + 1];
+    *seq = uniform(*seq);
+    *tok = uniform(*tok);
+    const int a = uniform(P.q_starts[*seq]), b = uniform(P.q_starts[*seq + 1]);
     if (a < 0 || b > P.n_tokens || *tok < 0 || b - a <= *tok) return false;
     *n = b - a - *tok < A.tok_tile ? b - a - *tok : A.tok_tile;
+    *row0 = a;
+    const int64_t pos = (int64_t)uniform(P.kv_lens[*seq]) - (b - a) + *tok;
+    *pos0 = (int)(pos < -(1 << 30) ? -(1 << 30) : pos);
     return true;
 }
 
@@ -84,30 +92,64 @@ __device__ __forceinline__ PagedRange paged_range(const PagedDev &P, const Paged
     return r;
 }
 
-// 8 codes of a K dword as exact halves c - 8, in the order nibble 0 4 1 5 2 6 3 7:
-// or-ing a nibble into 1024 (bits 0..3) or 64 (bits 4..7) makes the half 1024 + c
-// or 64 + c, so the dword needs one shift.
-__device__ __forceinline__ half8v paged_k8(uint32_t w) {
-    const half2v a = {(_Float16)-1032.0f, (_Float16)-1032.0f}, b = {(_Float16)-72.0f, (_Float16)-72.0f};
-    u32x4v r;
-    r[0] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, (w & 0x000F000Fu) | 0x64006400u) + a);
-    r[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, (w & 0x00F000F0u) | 0x54005400u) + b);
-    w >>= 8;
-    r[2] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, (w & 0x000F000Fu) | 0x64006400u) + a);
-    r[3] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2v, (w & 0x00F000F0u) | 0x54005400u) + b);
-    return __builtin_bit_cast(half8v, r);
-}
+__device__ __forceinline__ half2v paged_h2(uint32_t w) { return __builtin_bit_cast(half2v, w); }
 
-// bf16 pair (round to nearest even), low half first.
-__device__ __forceinline__ uint32_t paged_bf16x2(float a, float b) {
-    typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
-    bf16x2v r = {(__bf16)a, (__bf16)b};
-    return __builtin_bit_cast(uint32_t, r);
-}
+// Codes as exact halves c - 8: a nibble or-ed into 1024 (bits 0..3) or 64 (bits
+// 4..7) makes the half 1024 + c or 64 + c.  The two constants live in vector
+// registers of their own, so mask and or are one instruction (a VALU instruction
+// reads one scalar register or literal).
+struct PagedMagic {
+    uint32_t lo = 0x64006400u, hi = 0x54005400u;
+    __device__ __forceinline__ PagedMagic() { asm("" : "+v"(lo), "+v"(hi)); }
+    __device__ __forceinline__ uint32_t low(uint32_t w) const {
+        const half2v o = {(_Float16)-1032.0f, (_Float16)-1032.0f};
+        return __builtin_bit_cast(uint32_t, paged_h2((w & 0x000F000Fu) | lo) + o);
+    }
+    __device__ __forceinline__ uint32_t high(uint32_t w) const {
+        const half2v o = {(_Float16)-72.0f, (_Float16)-72.0f};
+        return __builtin_bit_cast(uint32_t, paged_h2((w & 0x00F000F0u) | hi) + o);
+    }
+    // the 8 codes of a K dword, in the order nibble 0 4 1 5 2 6 3 7
+    __device__ __forceinline__ half8v k8(uint32_t w) const {
+        const u32x4v r = {low(w), high(w), low(w >> 8), high(w >> 8)};
+        return __builtin_bit_cast(half8v, r);
+    }
+};
 
 template <int CTRL>
 __device__ __forceinline__ float paged_dpp(float v) {
     return __builtin_bit_cast(float, dpp_i<CTRL>(__builtin_bit_cast(int, v)));
+}
+// Where a wave's next 16 steps' tiles lie: lane j looks up tile j % 4 of the
+// wave's step j / 4.
+struct PagedWhere {
+    uint64_t codes;   // byte offset of the tile's codes
+    uint64_t scales;  // and of its scales
+    uint64_t ok;      // one bit per tile: inside the range, its page inside the pool
+};
+template <int G>
+__device__ __forceinline__ PagedWhere paged_where(const PagedDev &P, const PagedRange &rg, int seq, int64_t head_off,
+                                                  int step, int step_by, int s_hi) {
+    const int lane = threadIdx.x & 63;
+    const int s = step + (lane >> 2) * step_by;
+    const int t = rg.first + s * 64 + (lane & 3) * 16;
+    const bool in = s < s_hi && t < rg.hi;
+    int off = 0;
+    const int page = in ? paged_page(P, seq, t, &off) : -1;
+    if (page < 0) off = 0;
+    const uint64_t at = (uint64_t)(page < 0 ? 0 : page) * (uint64_t)(P.n_kv * P.block) + (uint64_t)head_off;
+    PagedWhere w;
+    w.codes = at + (uint32_t)off * (16 * G);
+    w.scales = at + (uint32_t)(P.ps * (16 * G) + off * (2 * G));
+    w.ok = __ballot(page >= 0);
+    return w;
+}
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int l) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l) |
+           (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), l) << 32;
+}
+__device__ __forceinline__ uint64_t shfl_u64(uint64_t v, int l) {
+    return (uint32_t)__shfl((int)(uint32_t)v, l, 64) | (uint64_t)(uint32_t)__shfl((int)(uint32_t)(v >> 32), l, 64) << 32;
 }
 
 // Row tiles of at most R = 4, 8 or 16 rows (tokens x query heads of one kv head):
@@ -117,58 +159,111 @@ __device__ __forceinline__ float paged_dpp(float v) {
 // the i-th of 16 / R tiles of 16 tokens: copy i's queries are zero in the other
 // columns, so the products of all tiles accumulate in one result whose lane
 // (column n, quarter c) holds the scores of row n % R against tokens 4 c + r of
-// tile n / R.  No lane's softmax work is spent on padding.  K codes stay integers:
-// each group's product is scaled by d of its (token, group) in f32.  For V the
-// scale goes into p (p d rounded to bf16, for f32 outputs in two terms), and the
-// codes are bf16 128 + c with a product against the constant -136 before each, so
-// the large offset never outlives a tile.
-template <int G, int R, bool F32>
-__global__ __launch_bounds__(256, G == 8 ? 1 : 2) void paged_attn_rows_kernel(PagedDev P, PagedAttn A) {
+// tile n / R.  No lane's softmax work is spent on padding.  Codes go into the
+// products as the exact integers c - 8; each group's K product is scaled by d of
+// its (token, group) in f32, and V's scale goes into p: p d 2^E as one half (two
+// for f32 rows: 22 bits), where E, the same for the wave, keeps the largest |d| seen
+// near 2^14, so p d leaves the normal halves only 2^28 below the largest.
+//
+// The W = 1 or 4 waves of a workgroup take a tile's steps in turn and join their
+// results.  Neighbouring workgroups are the kv heads of one tile, so the sessions
+// spread over the 8 XCDs (a session each made the XCD with the longest ones last).
+template <int G, int R, bool F32, int W>
+__global__ __launch_bounds__(64 * W, G == 8 ? 1 : G == 4 ? (R == 4 && !F32 ? 3 : 2) : R == 4 ? 4 : 3) void paged_attn_rows_kernel(PagedDev P, PagedAttn A) {
     constexpr int NT = 16 / R;  // token tiles per score result
     constexpr int NU = 4 / NT;  // score results per 64-token step
     constexpr int DV = 32 * G;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int col = lane & 15, quad = lane >> 4;
-    const int n_chunk = (A.kv_mul + 15) / 16;  // kv_mul > 16: 16 query heads at a time
-    const int kvh = blockIdx.y / n_chunk, h0 = (blockIdx.y % n_chunk) * 16;
-    const int heads = A.kv_mul - h0 < 16 ? A.kv_mul - h0 : 16;
-    const int split = blockIdx.z;
-    int seq, tok, n_tok;
-    if (!paged_tile(P, A, blockIdx.x, &seq, &tok, &n_tok)) return;
-    const int row0 = P.q_starts[seq];
-    const int64_t pos_end = P.kv_lens[seq];
-    const int64_t pos0l = pos_end - (P.q_starts[seq + 1] - row0) + tok;  // position of the tile's first token
-    const int pos0 = (int)(pos0l < -(1 << 30) ? -(1 << 30) : pos0l);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, quad = lane >> 4, copy = col / R;
+    const int heads_y = P.n_kv * A.n_chunk, tile = (int)(blockIdx.x / (uint32_t)heads_y);
+    const int head_y = (int)(blockIdx.x - (uint32_t)tile * (uint32_t)heads_y);
+    const int kvh = A.n_chunk == 1 ? head_y : head_y / A.n_chunk, h0 = A.n_chunk == 1 ? 0 : head_y % A.n_chunk * 16;
+    const bool last = A.kv_mul - h0 < 16;
+    const int heads = last ? A.kv_mul - h0 : 16, inv = last ? A.inv : A.inv16;
+    const int split = blockIdx.y;
+    int seq, tok, n_tok, row0, pos0;
+    if (!paged_tile(P, A, tile, &seq, &tok, &n_tok, &row0, &pos0)) return;
     const PagedRange rg = paged_range(P, A, pos0, n_tok);
 
+    // the splits' and then the waves' share of the steps
+    int per = A.split_steps;
+    if ((int64_t)per * A.n_splits < rg.steps) per = (rg.steps + A.n_splits - 1) / A.n_splits;
+    const int64_t s_at = (int64_t)split * per;
+    const int s_lo = (int)(s_at < rg.steps ? s_at : rg.steps);
+    const int s_hi = s_lo + per < rg.steps ? s_lo + per : rg.steps;
+    const int s_first = s_lo + wave;
+    const int n_mine = s_hi > s_first ? (s_hi - s_first + W - 1) / W : 0;  // steps s_first + W k
+    const int64_t head_off = (int64_t)kvh * P.block;
+    PagedWhere at = paged_where<G>(P, rg, seq, head_off, s_first, W, s_hi);
+
     // this lane's row: token and head of column col
-    const int row = col % R, my_tok = row / heads, my_head = row % heads;
+    const int row = col % R, my_tok = row * inv >> 8, my_head = row - my_tok * heads;
     const bool on = my_tok < n_tok;
     const int my_pos = pos0 + my_tok;
     int rhi = on ? my_pos + 1 : 0, rlo = A.window > 0 && my_pos - A.window + 1 > 0 ? my_pos - A.window + 1 : 0;
     if (rhi > rg.hi) rhi = rg.hi;
 
+    // Codes and scales of one step.  16-row tiles need every token's scales in every
+    // lane: those are loaded where they are used.
+    constexpr bool KEEP = R < 16;
+    uint32_t kc[4][G], vc[4][G], ks[KEEP ? NU : 1][2 * G], vs[KEEP ? NU : 1][2 * G];
+    const uint32_t k_lane = (uint32_t)((lane & 15) * 16 * G + quad * 4 * G);
+    const uint32_t v_lane = (uint32_t)(quad * 64 * G + (lane & 15) * 4 * G);
+    auto load_codes = [&](const uint8_t *pool, uint32_t mine, int k, uint32_t (&to)[4][G])
+                          __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            __builtin_memcpy(to[i], pool + lane_u64(at.codes, 4 * k + i) + mine, 4 * G);
+    };
+    auto scales_at = [&](int k, int u) __attribute__((always_inline)) {
+        return shfl_u64(at.scales, 4 * k + u * NT + copy) + (uint32_t)(quad * 8 * G);
+    };
+    auto load_k = [&](int k) __attribute__((always_inline)) {
+        load_codes(P.k, k_lane, k, kc);
+        if (KEEP)
+#pragma unroll
+            for (int u = 0; u < NU; u++) __builtin_memcpy(ks[KEEP ? u : 0], P.k + scales_at(k, u), 8 * G);
+    };
+    auto load_v = [&](int k) __attribute__((always_inline)) {
+        load_codes(P.v, v_lane, k, vc);
+        if (KEEP)
+#pragma unroll
+            for (int u = 0; u < NU; u++) __builtin_memcpy(vs[KEEP ? u : 0], P.v + scales_at(k, u), 8 * G);
+    };
+    if (n_mine > 0) {
+        load_k(0);
+        load_v(0);
+    }
+
     // queries: f16 of q 2^-e with 2^e above the row's largest (and the rest of it in
     // a second f16 for f32 inputs, 22 bits in all), zero in the other tiles' columns
-    half8v qh[NT][G], ql[F32 ? NT : 1][F32 ? G : 1];
+    // (in LDS where they would take 32 registers or more)
+    constexpr int TERMS = F32 ? 2 : 1;
+    constexpr bool QLDS = NT * G * TERMS >= 8;
+    half8v qr[QLDS ? 1 : TERMS][QLDS ? 1 : NT][QLDS ? 1 : G];
+    __shared__ half8v s_q[QLDS ? TERMS : 1][QLDS ? G : 1][QLDS ? 65 : 1];  // [lane], then zero
     float qf;
     {
         float x[G][8], big = 0.0f;
-        const int64_t at = (int64_t)(row0 + tok + my_tok) * A.q_stride + (int64_t)(kvh * A.kv_mul + h0 + my_head) * P.hd;
+        // a lane without a row or channel reads another's: the loads of all groups
+        // are in flight together, which a branch around each would prevent
+        const int64_t from = (int64_t)(row0 + tok + (on ? my_tok : 0)) * A.q_stride +
+                             (int64_t)(kvh * A.kv_mul + h0 + my_head) * P.hd;
 #pragma unroll
         for (int g = 0; g < G; g++) {
-            const int ch = 32 * g + 8 * quad;
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[g][j] = 0.0f;
-            if (on && ch < P.hd) {
-                if (F32) {
-                    row_load4((const float *)A.q + at + ch, x[g]);
-                    row_load4((const float *)A.q + at + ch + 4, x[g] + 4);
-                } else {
-                    row_load4((const uint16_t *)A.q + at + ch, x[g]);
-                    row_load4((const uint16_t *)A.q + at + ch + 4, x[g] + 4);
-                }
+            const int ch = 32 * g + 8 * quad, c = ch < P.hd ? ch : 0;
+            if (F32) {
+                row_load4((const float *)A.q + from + c, x[g]);
+                row_load4((const float *)A.q + from + c + 4, x[g] + 4);
+            } else {
+                row_load4((const uint16_t *)A.q + from + c, x[g]);
+                row_load4((const uint16_t *)A.q + from + c + 4, x[g] + 4);
             }
+        }
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[g][j] = on && 32 * g + 8 * quad < P.hd ? x[g][j] : 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; j++) big = fmaxf(big, fabsf(x[g][j]));
         }
@@ -177,76 +272,82 @@ __global__ __launch_bounds__(256, G == 8 ? 1 : 2) void paged_attn_rows_kernel(Pa
         int e = 0;
         if (big > 0.0f && big < __builtin_inff()) (void)frexpf(big, &e);
         qf = A.scale * ldexpf(1.0f, e);
+        const float down = ldexpf(1.0f, -(e >> 1)), more = ldexpf(1.0f, -(e - (e >> 1)));  // 2^-e may not be normal
         const int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
 #pragma unroll
         for (int g = 0; g < G; g++) {
+            if (QLDS && g % W != wave) continue;  // a wave each
             half8v hi, lo;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float v = ldexpf(x[g][order[j]], -e);
+                const float v = x[g][order[j]] * down * more;
                 hi[j] = (_Float16)v;
                 lo[j] = (_Float16)(v - (float)hi[j]);
             }
             const half8v zero = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (!QLDS) {
 #pragma unroll
-            for (int i = 0; i < NT; i++) {
-                qh[i][g] = col / R == i ? hi : zero;
-                if (F32) ql[i][g] = col / R == i ? lo : zero;
+                for (int i = 0; i < NT; i++) {
+                    qr[0][QLDS ? 0 : i][QLDS ? 0 : g] = copy == i ? hi : zero;
+                    if (F32) qr[QLDS ? 0 : TERMS - 1][QLDS ? 0 : i][QLDS ? 0 : g] = copy == i ? lo : zero;
+                }
+            } else {
+                half8v *to = s_q[0][QLDS ? g : 0];
+                to[lane] = hi;
+                if (lane == 0) to[64] = zero;
+                if (F32) {
+                    to = s_q[QLDS ? TERMS - 1 : 0][QLDS ? g : 0];
+                    to[lane] = lo;
+                    if (lane == 0) to[64] = zero;
+                }
             }
         }
     }
+    if (QLDS) __syncthreads();
 
-    // the splits' and then the waves' share of the steps
-    int per = A.split_steps;
-    if ((int64_t)per * A.n_splits < rg.steps) per = (rg.steps + A.n_splits - 1) / A.n_splits;
-    const int s_lo = split * per < rg.steps ? split * per : rg.steps;
-    const int s_hi = s_lo + per < rg.steps ? s_lo + per : rg.steps;
-
-    float m = -__builtin_inff(), l = 0.0f;
+    float m = -__builtin_inff(), l = 0.0f, E = 0.0f, d2_most = 0.0f;
     f32x4v acc[G][2];
 #pragma unroll
     for (int g = 0; g < G; g++)
 #pragma unroll
         for (int h = 0; h < 2; h++) acc[g][h] = f32x4v{0, 0, 0, 0};
-    u32x4v bias_u = {0xC308C308u, 0xC308C308u, 0xC308C308u, 0xC308C308u};
-    const bf16x8v bias = __builtin_bit_cast(bf16x8v, bias_u);
-
     // rows whose masks the whole step passes need no masking
     const int full_lo = rg.lo + (A.window > 0 ? n_tok - 1 : 0), full_hi = rg.hi - (n_tok - 1);
-    const uint32_t k_lane = (uint32_t)((lane & 15) * 16 * G + quad * 4 * G);
-    const uint32_t v_lane = (uint32_t)(quad * 64 * G + (lane & 15) * 4 * G);
-    const int64_t head_off = (int64_t)kvh * P.block, page_bytes = (int64_t)P.n_kv * P.block;
 
-    for (int s = s_lo + wave; s < s_hi; s += 4) {
-        const int t0 = rg.first + s * 64;
-        uint32_t kc[4][G], vc[4][G], ks[NU][2 * G], vs[NU][2 * G];
-        int pg[4];
+    const PagedMagic magic;
+    for (int k = 0; k < n_mine; k++) {
+        const int t0 = rg.first + (s_first + W * k) * 64;
+        const uint32_t okm = (uint32_t)(at.ok >> (4 * (k & 15))) & 15;
+        const bool full = t0 >= full_lo && t0 + 64 <= full_hi && okm == 15, more = k + 1 < n_mine;
+        // what this lane's row does not see may hold anything: its scales become 0
+        auto clear = [&](int u, uint32_t (&d)[2 * G]) __attribute__((always_inline)) {
+            const bool page = (okm >> (u * NT + copy)) & 1;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int t = t0 + 16 * i;
-            pg[i] = t < rg.hi ? __builtin_amdgcn_readfirstlane(paged_page(P, seq, t)) : -1;
-            const int64_t at = (int64_t)(pg[i] < 0 ? 0 : pg[i]) * page_bytes + head_off + (int64_t)(t % P.ps) * (16 * G);
-            __builtin_memcpy(kc[i], P.k + at + k_lane, 4 * G);
-            __builtin_memcpy(vc[i], P.v + at + v_lane, 4 * G);
-        }
+            for (int r = 0; r < 4; r++) {
+                const int t = t0 + 16 * (u * NT + copy) + 4 * quad + r;
+                const bool out = t < rlo || t >= rhi || !page;
 #pragma unroll
-        for (int u = 0; u < NU; u++) {
-            int page = pg[u * NT];
-#pragma unroll
-            for (int i = 1; i < NT; i++) page = col / R == i ? pg[u * NT + i] : page;
-            const int t = t0 + 16 * (u * NT + col / R) + 4 * quad;
-            const int64_t at = (int64_t)(page < 0 ? 0 : page) * page_bytes + head_off + (int64_t)P.ps * (16 * G) +
-                               (int64_t)(t % P.ps) * (2 * G);
-            __builtin_memcpy(ks[u], P.k + at, 8 * G);
-            __builtin_memcpy(vs[u], P.v + at, 8 * G);
-        }
-        const bool full = t0 >= full_lo && t0 + 64 <= full_hi && pg[0] >= 0 && pg[1] >= 0 && pg[2] >= 0 && pg[3] >= 0;
+                for (int g = 0; g < G; g++) {
+                    const int e = r * G + g;
+                    d[e >> 1] &= out ? (e & 1 ? 0x0000FFFFu : 0xFFFF0000u) : 0xFFFFFFFFu;
+                }
+            }
+        };
 
         // scores
-        float sc[NU][4];
-        float mx = -__builtin_inff();
+        int q_at = lane;
+        asm volatile("" : "+v"(q_at));  // keeps the reads in the loop, out of registers before it
+        auto query = [&](int term, int i, int g) __attribute__((always_inline)) {
+            if (QLDS)
+                return s_q[QLDS ? term : 0][QLDS ? g : 0][QLDS ? (copy == i ? q_at : 64) : 0];
+            return qr[QLDS ? 0 : term][QLDS ? 0 : i][QLDS ? 0 : g];
+        };
+        float sc[NU][4], mx = -__builtin_inff();
 #pragma unroll
         for (int u = 0; u < NU; u++) {
+            uint32_t late[2 * G];
+            if (!KEEP) __builtin_memcpy(late, P.k + scales_at(k & 15, u), 8 * G);
+            const uint32_t(&kd)[2 * G] = KEEP ? ks[KEEP ? u : 0] : late;
 #pragma unroll
             for (int r = 0; r < 4; r++) sc[u][r] = 0.0f;
 #pragma unroll
@@ -254,40 +355,64 @@ __global__ __launch_bounds__(256, G == 8 ? 1 : 2) void paged_attn_rows_kernel(Pa
                 f32x4v d = {0, 0, 0, 0};
 #pragma unroll
                 for (int i = 0; i < NT; i++) {
-                    const half8v k8 = paged_k8(kc[u * NT + i][g]);
-                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qh[i][g], d, 0, 0, 0);
-                    if (F32) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, ql[i][g], d, 0, 0, 0);
+                    const half8v k8 = magic.k8(kc[u * NT + i][g]);
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, query(0, i, g), d, 0, 0, 0);
+                    if (F32) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, query(TERMS - 1, i, g), d, 0, 0, 0);
                 }
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int e = r * G + g;
-                    const float f = h2f((uint16_t)(ks[u][e >> 1] >> (16 * (e & 1))));
-                    sc[u][r] = fmaf(f, d[r], sc[u][r]);
+                    sc[u][r] = fmaf((float)paged_h2(kd[e >> 1])[e & 1], d[r], sc[u][r]);
                 }
             }
 #pragma unroll
             for (int r = 0; r < 4; r++) sc[u][r] *= qf;
             if (!full) {
-                int page = pg[u * NT];
-#pragma unroll
-                for (int i = 1; i < NT; i++) page = col / R == i ? pg[u * NT + i] : page;
+                const bool page = (okm >> (u * NT + copy)) & 1;
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int t = t0 + 16 * (u * NT + col / R) + 4 * quad + r;
-                    if (t < rlo || t >= rhi || page < 0) sc[u][r] = -__builtin_inff();
+                    const int t = t0 + 16 * (u * NT + copy) + 4 * quad + r;
+                    if (t < rlo || t >= rhi || !page) sc[u][r] = -__builtin_inff();
                 }
             }
 #pragma unroll
             for (int r = 0; r < 4; r++) mx = fmaxf(mx, sc[u][r]);
         }
-        if (__ballot(mx > m)) {
+        // the registers are free again: the next step's keys, under this one's values
+        // (the last step loads its own again: with a branch around them the waits for
+        // the values would count these loads as well)
+        if (KEEP) {
+            if (more && ((k + 1) & 15) == 0)
+                at = paged_where<G>(P, rg, seq, head_off, s_first + W * (k + 1), W, s_hi);
+            load_k((more ? k + 1 : k) & 15);
+        }
+
+        float d2 = 0.0f;
+#pragma unroll
+        for (int u = 0; u < NU; u++) {
+            uint32_t late[2 * G];
+            if (!KEEP) __builtin_memcpy(late, P.v + scales_at(k & 15, u), 8 * G);
+            uint32_t(&vd)[2 * G] = KEEP ? vs[KEEP ? u : 0] : late;
+            if (!full) clear(u, vd);
+#pragma unroll
+            for (int j = 0; j < 2 * G; j++) d2 = __builtin_amdgcn_fdot2(paged_h2(vd[j]), paged_h2(vd[j]), d2, false);
+        }
+        if (__ballot(mx > m || d2 > d2_most)) {
             // a row's scores lie in the lanes of all tiles and quarters
             if (NT >= 4) mx = fmaxf(mx, paged_dpp<0x124>(mx));
             if (NT >= 2) mx = fmaxf(mx, paged_dpp<0x128>(mx));
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             mx = fmaxf(mx, m);
-            const float a = m == mx ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
+            d2 = wave_max(d2);
+            const float was = m - E;
+            if (d2 > d2_most) {
+                int e;
+                (void)frexpf(d2, &e);  // |d| <= 2^(e / 2)
+                E = (float)(14 - ((e + 1) >> 1));
+                d2_most = ldexpf(1.0f, 2 * (15 - (int)E));
+            }
+            const float a = m == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(was - (mx - E));
             m = mx;
             l *= a;
 #pragma unroll
@@ -295,7 +420,7 @@ __global__ __launch_bounds__(256, G == 8 ? 1 : 2) void paged_attn_rows_kernel(Pa
 #pragma unroll
                 for (int h = 0; h < 2; h++) acc[g][h] *= a;
         }
-        const float base = m == -__builtin_inff() ? 0.0f : m;
+        const float base = (m == -__builtin_inff() ? 0.0f : m) - E;
 #pragma unroll
         for (int u = 0; u < NU; u++)
 #pragma unroll
@@ -306,47 +431,50 @@ __global__ __launch_bounds__(256, G == 8 ? 1 : 2) void paged_attn_rows_kernel(Pa
 
         // values, 32 tokens (two tiles) per product
 #pragma unroll
-        for (int g = 0; g < G; g++) {
-            uint32_t ph[NU][2], pl[NU][2];
+        for (int k2 = 0; k2 < 2; k2++) {
+            constexpr int UU = NU > 1 ? NU / 2 : 1;  // score results of these 32 tokens
+            uint32_t late[2][2 * G];
+            if (!KEEP)
 #pragma unroll
-            for (int u = 0; u < NU; u++) {
-                float f[4];
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int e = r * G + g;
-                    f[r] = sc[u][r] * h2f((uint16_t)(vs[u][e >> 1] >> (16 * (e & 1))));
-                    // a masked token's page may hold anything, NaN among it
-                    if (!full) f[r] = sc[u][r] == 0.0f ? 0.0f : f[r];
+                for (int x = 0; x < 2; x++) {
+                    __builtin_memcpy(late[x], P.v + scales_at(k & 15, 2 * k2 + x), 8 * G);
+                    if (!full) clear(2 * k2 + x, late[x]);
                 }
-                ph[u][0] = paged_bf16x2(f[0], f[1]);
-                ph[u][1] = paged_bf16x2(f[2], f[3]);
-                if (F32) {
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const uint32_t w = ph[u][r >> 1];
-                        f[r] -= __builtin_bit_cast(float, r & 1 ? w & 0xFFFF0000u : w << 16);
+            for (int g = 0; g < G; g++) {
+                uint32_t ph[UU][2], pl[UU][2];
+#pragma unroll
+                for (int v = 0; v < UU; v++)
+#pragma unroll
+                    for (int r = 0; r < 4; r += 2) {
+                        const int u = NU > 1 ? k2 * UU + v : 0;
+                        half2v hi, lo;
+#pragma unroll
+                        for (int x = 0; x < 2; x++) {
+                            const int e = (r + x) * G + g;
+                            const uint32_t w = KEEP ? vs[KEEP ? u : 0][e >> 1] : late[v & 1][e >> 1];
+                            const _Float16 d = paged_h2(w)[e & 1];
+                            hi[x] = (_Float16)fmaf(sc[u][r + x], (float)d, 0.0f);
+                            if (F32) lo[x] = (_Float16)fmaf(sc[u][r + x], (float)d, -(float)hi[x]);
+                        }
+                        ph[v][r >> 1] = __builtin_bit_cast(uint32_t, hi);
+                        if (F32) pl[v][r >> 1] = __builtin_bit_cast(uint32_t, lo);
                     }
-                    pl[u][0] = paged_bf16x2(f[0], f[1]);
-                    pl[u][1] = paged_bf16x2(f[2], f[3]);
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
                 u32x4v bh, bl = {0, 0, 0, 0};
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
-                    const int i = (2 * k + x) % NT, u = (2 * k + x) / NT;
+                    const int i = (2 * k2 + x) % NT, v = NU > 1 ? (2 * k2 + x) / NT - k2 * UU : 0;
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         // copy i's columns to the first R (row_ror by 16 - R i)
-                        auto turn = [&](uint32_t v) -> uint32_t {
-                            if (i == 0) return v;
-                            if (i * R == 4) return (uint32_t)dpp_i<0x12C>((int)v);
-                            if (i * R == 8) return (uint32_t)dpp_i<0x128>((int)v);
-                            return (uint32_t)dpp_i<0x124>((int)v);
+                        auto turn = [&](uint32_t y) -> uint32_t {
+                            if (i == 0) return y;
+                            if (i * R == 4) return (uint32_t)dpp_i<0x12C>((int)y);
+                            if (i * R == 8) return (uint32_t)dpp_i<0x128>((int)y);
+                            return (uint32_t)dpp_i<0x124>((int)y);
                         };
-                        bh[2 * x + h] = turn(ph[u][h]);
-                        if (F32) bl[2 * x + h] = turn(pl[u][h]);
+                        bh[2 * x + h] = turn(ph[v][h]);
+                        if (F32) bl[2 * x + h] = turn(pl[v][h]);
                     }
                 }
                 u32x4v va, vb;
@@ -355,67 +483,73 @@ __global__ __launch_bounds__(256, G == 8 ? 1 : 2) void paged_attn_rows_kernel(Pa
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         const int b0 = (2 * h) * G + g, b1 = (2 * h + 1) * G + g;
-                        const uint32_t w = __builtin_amdgcn_perm(vc[2 * k + x][b1 >> 2], vc[2 * k + x][b0 >> 2],
+                        const uint32_t w = __builtin_amdgcn_perm(vc[2 * k2 + x][b1 >> 2], vc[2 * k2 + x][b0 >> 2],
                                                                  0x0C000C00u | (uint32_t)(b0 & 3) |
                                                                      (uint32_t)(4 + (b1 & 3)) << 16);
-                        va[2 * x + h] = (w & 0x000F000Fu) | 0x43004300u;
-                        vb[2 * x + h] = ((w >> 4) & 0x000F000Fu) | 0x43004300u;
+                        va[2 * x + h] = magic.low(w);
+                        vb[2 * x + h] = magic.high(w);
                     }
-                const bf16x8v p8 = __builtin_bit_cast(bf16x8v, bh);
+                const half8v p8 = __builtin_bit_cast(half8v, bh);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const bf16x8v v8 = __builtin_bit_cast(bf16x8v, h ? vb : va);
-                    acc[g][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bias, p8, acc[g][h], 0, 0, 0);
-                    acc[g][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v8, p8, acc[g][h], 0, 0, 0);
-                    if (F32) {
-                        const bf16x8v l8 = __builtin_bit_cast(bf16x8v, bl);
-                        acc[g][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bias, l8, acc[g][h], 0, 0, 0);
-                        acc[g][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v8, l8, acc[g][h], 0, 0, 0);
-                    }
+                    const half8v v8 = __builtin_bit_cast(half8v, h ? vb : va);
+                    acc[g][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, p8, acc[g][h], 0, 0, 0);
+                    if (F32)
+                        acc[g][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, __builtin_bit_cast(half8v, bl),
+                                                                           acc[g][h], 0, 0, 0);
                 }
             }
         }
+        if (!KEEP) {
+            if (more && ((k + 1) & 15) == 0)
+                at = paged_where<G>(P, rg, seq, head_off, s_first + W * (k + 1), W, s_hi);
+            load_k((more ? k + 1 : k) & 15);
+        }
+        load_v((more ? k + 1 : k) & 15);
     }
 
-    // the four waves' results through LDS
+    // the lanes' results through LDS, and the waves' joined
     if (NT >= 4) l += paged_dpp<0x124>(l);
     if (NT >= 2) l += paged_dpp<0x128>(l);
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
-    __shared__ float s_acc[4][R][DV + 4];
-    __shared__ float s_m[4][R], s_l[4][R];
+    const float unit = ldexpf(1.0f, -(int)E);
+    __shared__ float s_acc[W][R][DV + 4];
+    __shared__ float s_m[W][R], s_l[W][R];
     if (col < R) {
         if (quad == 0) {
             s_m[wave][col] = m;
-            s_l[wave][col] = l;
+            s_l[wave][col] = l * unit;
         }
 #pragma unroll
         for (int g = 0; g < G; g++)
 #pragma unroll
             for (int h = 0; h < 2; h++)
-                *(f32x4v *)&s_acc[wave][col][32 * g + 16 * h + 4 * quad] = acc[g][h];
+                *(f32x4v *)&s_acc[wave][col][32 * g + 16 * h + 4 * quad] = acc[g][h] * unit;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < R * DV; i += 256) {
+    for (int i = threadIdx.x; i < R * DV; i += 64 * W) {
         const int r = i / DV, ch = i % DV;
-        const int tk = r / heads, hd = kvh * A.kv_mul + h0 + r % heads;
+        const int tk = r * inv >> 8, hd = kvh * A.kv_mul + h0 + r - tk * heads;
         if (tk >= n_tok) break;
-        float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+        float top = s_m[0][r];
+#pragma unroll
+        for (int w = 1; w < W; w++) top = fmaxf(top, s_m[w][r]);
         const float base = top == -__builtin_inff() ? 0.0f : top;
         float sum = 0.0f, o = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < W; w++) {
             const float f = __builtin_amdgcn_exp2f(s_m[w][r] - base);
             sum = fmaf(f, s_l[w][r], sum);
             o = fmaf(f, s_acc[w][r][ch], o);
         }
         const int64_t token = row0 + tok + tk;
         if (A.n_splits > 1) {
-            const int64_t at = ((int64_t)split * P.n_tokens + token) * A.n_heads + hd;
-            if (top != -__builtin_inff()) A.part[at * DV + ch] = o;
+            const int64_t to = ((int64_t)split * P.n_tokens + token) * A.n_heads + hd;
+            if (top != -__builtin_inff()) A.part[to * DV + ch] = o;
             if (ch == 0) {
-                A.ml[at * 2] = top;
-                A.ml[at * 2 + 1] = sum;
+                A.ml[to * 2] = top;
+                A.ml[to * 2 + 1] = sum;
             }
             continue;
         }
@@ -423,12 +557,8 @@ __global__ __launch_bounds__(256, G == 8 ? 1 : 2) void paged_attn_rows_kernel(Pa
         if (A.sinks) {
             const float sink = A.sinks[hd] * 1.44269504f;
             const float to = fmaxf(base, sink), f = __builtin_amdgcn_exp2f(base - to);
-            if (top == -__builtin_inff()) {
-                o = 0.0f, sum = 1.0f;
-            } else {
-                sum = fmaf(sum, f, __builtin_amdgcn_exp2f(sink - to));
-                o *= f;
-            }
+            sum = fmaf(sum, f, __builtin_amdgcn_exp2f(sink - to));
+            o *= f;
         }
         const float y = top == -__builtin_inff() ? 0.0f : o / sum;
         const int64_t to = token * A.o_stride + (int64_t)hd * P.vd + ch;
@@ -439,47 +569,61 @@ __global__ __launch_bounds__(256, G == 8 ? 1 : 2) void paged_attn_rows_kernel(Pa
     }
 }
 
-// Joins a row's splits in their order.  One wave per (token, query head).
+// Joins a row's splits.  One workgroup per (token, query head): the splits'
+// weights first, then each of 256 / DV groups of threads sums every so-manieth
+// split, eight loads in flight, and the groups' sums are added in their order.
 template <int G, bool F32>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedDev P, PagedAttn A) {
-    constexpr int DV = 32 * G;
-    const int lane = threadIdx.x & 63;
-    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int64_t rows = (int64_t)P.n_tokens * A.n_heads;
-    if (w >= rows) return;
+    constexpr int DV = 32 * G, N = 256 / DV;
+    __shared__ float s_f[256], s_o[N][DV], s_red[4];
+    const int64_t rows = (int64_t)P.n_tokens * A.n_heads, w = blockIdx.x;
     const int token = (int)(w / A.n_heads), hd = (int)(w % A.n_heads);
+    const int i = threadIdx.x;  // n_splits <= 256
+    float m = -__builtin_inff(), part = 0.0f;
+    if (i < A.n_splits) {
+        m = A.ml[(i * rows + w) * 2];
+        part = A.ml[(i * rows + w) * 2 + 1];
+    }
     int seq, a, b;
     // rows of no tile stay as they are
     if (!paged_session(P, token, &seq, &a, &b) || (A.by_seq && token - a >= A.tok_tile)) return;
-    float top = -__builtin_inff();
-    for (int s = 0; s < A.n_splits; s++) top = fmaxf(top, A.ml[(s * rows + w) * 2]);
+    const float top = block_max_256(m, s_red);
     const bool none = top == -__builtin_inff();
-    float base = none ? 0.0f : top, sum = 0.0f;
+    float base = none ? 0.0f : top, sink = 0.0f;
     if (A.sinks) {
-        const float sink = A.sinks[hd] * 1.44269504f;
+        sink = A.sinks[hd] * 1.44269504f;
         base = none ? sink : fmaxf(base, sink);
-        sum = __builtin_amdgcn_exp2f(sink - base);
+        sink = __builtin_amdgcn_exp2f(sink - base);
     }
-    float o[DV / 64] = {};
-    for (int s = 0; s < A.n_splits; s++) {
-        const float m = A.ml[(s * rows + w) * 2];
-        if (m == -__builtin_inff()) continue;
-        const float f = __builtin_amdgcn_exp2f(m - base);
-        sum = fmaf(f, A.ml[(s * rows + w) * 2 + 1], sum);
+    const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - base);
+    s_f[i] = f;
+    const float sum = block_sum_256(f == 0.0f ? 0.0f : f * part, s_red) + sink;  // the barriers order s_f too
+    const int ch = i % DV;
+    float o[4] = {0, 0, 0, 0};
+    for (int s = i / DV; s < A.n_splits; s += 8 * N) {
+        float x[8], f8[8];
 #pragma unroll
-        for (int j = 0; j < DV / 64; j++) o[j] = fmaf(f, A.part[(s * rows + w) * DV + lane + 64 * j], o[j]);
-    }
+        for (int j = 0; j < 8; j++) {
+            const int at = s + j * N < A.n_splits ? s + j * N : 0;
+            f8[j] = s + j * N < A.n_splits ? s_f[at] : 0.0f;
+            x[j] = A.part[(at * rows + w) * DV + ch];
+        }
 #pragma unroll
-    for (int j = 0; j < DV / 64; j++) {
-        const int ch = lane + 64 * j;
-        if (ch >= P.vd) continue;
-        const float y = none ? 0.0f : o[j] / sum;
-        const int64_t to = token * A.o_stride + (int64_t)hd * P.vd + ch;
-        if (F32)
-            ((float *)A.out)[to] = y;
-        else
-            ((uint16_t *)A.out)[to] = f32_to_bf16(y);
+        for (int j = 0; j < 8; j++)  // a split without keys wrote no sums
+            o[j & 3] = f8[j] != 0.0f ? fmaf(f8[j], x[j], o[j & 3]) : o[j & 3];
     }
+    s_o[i / DV][ch] = (o[0] + o[1]) + (o[2] + o[3]);
+    __syncthreads();
+    if (i >= DV || ch >= P.vd) return;
+    float y = s_o[0][ch];
+#pragma unroll
+    for (int j = 1; j < N; j++) y += s_o[j][ch];
+    y = none ? 0.0f : y / sum;
+    const int64_t to = token * A.o_stride + (int64_t)hd * P.vd + ch;
+    if (F32)
+        ((float *)A.out)[to] = y;
+    else
+        ((uint16_t *)A.out)[to] = f32_to_bf16(y);
 }
 
 }  // namespace rh

@@ -4436,6 +4436,11 @@ static bool paged_dev(const RustyPagedKv *kv, const RustyPagedBatch *b, PagedDev
     P->stride = (int)b->table_stride;
     P->n_tokens = (int)b->n_rows;
     P->block = (int64_t)kv->page_size * 18 * paged_groups(kv->head_dim, kv->value_dim);
+    const uint32_t tiles = kv->page_size / 16;
+    uint32_t log = 0;
+    while ((1u << log) < tiles) log++;
+    P->tile_shift = 31 + log;
+    P->tile_mul = tiles == 1 ? 0 : (uint32_t)(((1ull << P->tile_shift) + tiles - 1) / tiles);
     return true;
 }
 
@@ -4463,13 +4468,13 @@ struct PagedDevice {
     }
 };
 
-// How a call's attention is cut: rows per tile, tiles, and splits of a tile's
-// cached range.
+// How a call's attention is cut: rows per tile, waves per tile, and splits of a
+// tile's cached range.
 struct PagedPlan {
-    int R, tok_tile, by_seq, n_splits, split_steps;
+    int R, W, tok_tile, by_seq, n_splits, split_steps;
     int64_t tiles, heads_y;
 };
-static PagedPlan paged_plan(const PagedDev &P, uint32_t n_heads, uint32_t max_q, uint32_t max_kv) {
+static PagedPlan paged_plan(const PagedDev &P, uint32_t n_heads, uint32_t max_q, uint32_t max_kv, uint32_t window) {
     PagedPlan p;
     const int kv_mul = (int)n_heads / P.n_kv, chunk = kv_mul < 16 ? kv_mul : 16;
     const bool wide = P.hd > 128 || P.vd > 128;  // 4-row tiles there would not fit the registers
@@ -4479,15 +4484,24 @@ static PagedPlan paged_plan(const PagedDev &P, uint32_t n_heads, uint32_t max_q,
     p.by_seq = max_q <= (uint32_t)p.tok_tile;
     p.tiles = p.by_seq ? P.n_seqs : P.n_tokens / p.tok_tile + (int64_t)P.n_seqs;
     p.heads_y = (int64_t)P.n_kv * ((kv_mul + 15) / 16);
-    const int64_t steps = ((int64_t)max_kv + 15 + 63) / 64 + 1;
-    // a workgroup takes four steps at a time; enough of them for four per CU
-    int64_t splits = (4 * 256 + p.tiles * p.heads_y - 1) / (p.tiles * p.heads_y);
-    const int64_t most = (steps + 3) / 4;
-    if (splits > most) splits = most;
-    if (splits > 256) splits = 256;
-    if (splits < 1) splits = 1;
-    p.n_splits = (int)splits;
-    p.split_steps = (int)((steps + splits - 1) / splits);
+    int64_t seen = max_kv;
+    if (window && (int64_t)window + p.tok_tile + 15 < seen) seen = (int64_t)window + p.tok_tile + 15;
+    const int64_t steps = seen > 0 ? (seen + 63) / 64 : 1, items = p.tiles * p.heads_y;
+    // Eight waves per CU or more of short (tile, kv head) pairs: a wave each (256
+    // sessions of 128 positions, 8 kv heads: 15.0 us, 16.8 with a workgroup each).
+    // Otherwise a workgroup each, and splits of 4 to 64 steps (1 to 16 per wave) for
+    // three workgroups per CU: 48 ragged sessions of up to 8192 take 76 us with 64
+    // steps, 80 with 16; one of 131072 takes 36 and 43.
+    p.W = items >= 2048 && steps <= 16 ? 1 : 4;
+    int64_t per = 16;
+    if (p.W == 4) {
+        per = (steps * items + 767) / 768;
+        per = per < 4 ? 4 : per > 64 ? 64 : per;
+    }
+    if (steps <= per + per / 2) per = steps;
+    if ((steps + per - 1) / per > 256) per = (steps + 255) / 256;
+    p.n_splits = (int)((steps + per - 1) / per);
+    p.split_steps = (int)per;
     return p;
 }
 static uint64_t paged_workspace(const PagedDev &P, const PagedPlan &p, uint32_t n_heads) {
@@ -4498,19 +4512,24 @@ static bool paged_heads_ok(const PagedDev &P, uint32_t n_heads) {
     return n_heads && n_heads <= 65536 && n_heads % P.n_kv == 0;
 }
 
+template <int G, bool F32, int W>
+static void paged_attn_rows_launch(const PagedDev &P, const PagedAttn &A, const PagedPlan &p, hipStream_t s) {
+    const dim3 grid((unsigned)(p.tiles * p.heads_y), (unsigned)p.n_splits);
+    if (p.R == 16)
+        paged_attn_rows_kernel<G, 16, F32, W><<<grid, 64 * W, 0, s>>>(P, A);
+    else if (p.R == 8)
+        paged_attn_rows_kernel<G, 8, F32, W><<<grid, 64 * W, 0, s>>>(P, A);
+    else if constexpr (G != 8)
+        paged_attn_rows_kernel<G, 4, F32, W><<<grid, 64 * W, 0, s>>>(P, A);
+}
 template <int G, bool F32>
 static void paged_attn_launch(const PagedDev &P, const PagedAttn &A, const PagedPlan &p, hipStream_t s) {
-    const dim3 grid((unsigned)p.tiles, (unsigned)p.heads_y, (unsigned)p.n_splits);
-    if (p.R == 16)
-        paged_attn_rows_kernel<G, 16, F32><<<grid, 256, 0, s>>>(P, A);
-    else if (p.R == 8)
-        paged_attn_rows_kernel<G, 8, F32><<<grid, 256, 0, s>>>(P, A);
-    else if constexpr (G != 8)
-        paged_attn_rows_kernel<G, 4, F32><<<grid, 256, 0, s>>>(P, A);
-    if (p.n_splits > 1) {
-        const int64_t rows = (int64_t)P.n_tokens * A.n_heads;
-        paged_attn_join_kernel<G, F32><<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(P, A);
-    }
+    if (p.W == 1)
+        paged_attn_rows_launch<G, F32, 1>(P, A, p, s);
+    else
+        paged_attn_rows_launch<G, F32, 4>(P, A, p, s);
+    if (p.n_splits > 1)
+        paged_attn_join_kernel<G, F32><<<(unsigned)((int64_t)P.n_tokens * A.n_heads), 256, 0, s>>>(P, A);
 }
 
 }  // namespace rh
@@ -4630,7 +4649,7 @@ uint64_t rusty_hip_paged_attention_workspace(const RustyPagedKv *kv, const Rusty
     using namespace rh;
     PagedDev P;
     if (!paged_dev(kv, batch, &P, true) || !paged_heads_ok(P, n_heads)) return 0;
-    return paged_workspace(P, paged_plan(P, n_heads, batch->max_q_len, batch->max_kv_len), n_heads);
+    return paged_workspace(P, paged_plan(P, n_heads, batch->max_q_len, batch->max_kv_len, 0), n_heads);
 }
 
 int rusty_hip_paged_attention(const RustyPagedKv *kv, const RustyPagedBatch *batch, const RustyPagedAttention *rows,
@@ -4647,10 +4666,10 @@ int rusty_hip_paged_attention(const RustyPagedKv *kv, const RustyPagedBatch *bat
         return 0;
     PagedDevice dev((hipStream_t)stream);
     if (!dev.ok) return 0;
-    const PagedPlan p = paged_plan(P, rows->n_heads, batch->max_q_len, batch->max_kv_len);
+    const PagedPlan p = paged_plan(P, rows->n_heads, batch->max_q_len, batch->max_kv_len, rows->window);
     const uint64_t need = paged_workspace(P, p, rows->n_heads);
     if (need && (!rows->workspace || rows->workspace_len < need || (uintptr_t)rows->workspace % 16)) return 0;
-    if (p.tiles > 0x7FFFFFFF || p.heads_y > 65535 || ((int64_t)n * rows->n_heads + 3) / 4 > 0x7FFFFFFF) return 0;
+    if (p.tiles * p.heads_y > (0x7FFFFFFF >> 8) || (int64_t)n * rows->n_heads > 0x7FFFFFFF) return 0;
     PagedAttn A;
     A.q = rows->q;
     A.out = rows->out;
@@ -4662,6 +4681,9 @@ int rusty_hip_paged_attention(const RustyPagedKv *kv, const RustyPagedBatch *bat
     A.scale = rows->scale * 1.44269504f;
     A.n_heads = (int)rows->n_heads;
     A.kv_mul = (int)rows->n_heads / P.n_kv;
+    A.n_chunk = (A.kv_mul + 15) / 16;
+    A.inv16 = 16;
+    A.inv = (A.kv_mul & 15) ? (256 + (A.kv_mul & 15) - 1) / (A.kv_mul & 15) : 16;
     A.window = (int)rows->window;
     A.tok_tile = p.tok_tile;
     A.n_splits = p.n_splits;
