@@ -11,6 +11,8 @@
 
 namespace rh {
 
+typedef float f32x16v __attribute__((ext_vector_type(16)));
+
 struct PagedAttn {
     const void *q;
     void *out;
@@ -25,54 +27,53 @@ struct PagedAttn {
     int32_t tok_tile;    // tokens of a row tile
     int32_t n_splits;    // most splits of a row tile's range
     int32_t split_steps; // 64-token steps of a split, more where n_splits would not cover the range
-    int32_t by_seq;      // 1: tile x is session x (at most one tile each)
+    int32_t short_q;     // sessions of up to so many rows are row tiles of their own (paged_attn_rows_kernel)
+    int32_t both;        // 1: the others are paged_attn_tile_kernel's; 0: all are of one kind
+    int32_t tile_splits; // n_splits of the others (for the join)
 };
 
-// Row tile x of the batch: its session, first token (of the session) and tokens, the
-// session's first row, and the first token's position.  Wave-uniform; 64 sessions
-// per turn, each lane one session's tile count.
-__device__ __forceinline__ bool paged_tile(const PagedDev &P, const PagedAttn &A, int x, int *seq, int *tok, int *n,
-                                           int *row0, int *pos0) {
-    const int lane = threadIdx.x & 63;
-    if (A.by_seq) {
-        *seq = x;
-        *tok = 0;
-    } else {
-        int before = 0, found = -1;
-        for (int base = 0; base < P.n_seqs; base += 64) {
-            const int i = base + lane;
-            int c = 0;
-            if (i < P.n_seqs) {
-                const int64_t len = (int64_t)P.q_starts[i + 1] - P.q_starts[i];
-                c = len > 0 && len <= P.n_tokens ? ((int)len + A.tok_tile - 1) / A.tok_tile : 0;
-            }
-            int sum = c;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int up = __shfl_up(sum, o, 64);
-                if (lane >= o) sum += up;
-            }
-            const uint64_t here = __ballot(before + sum > x);
-            if (here) {
-                const int l = __ffsll((unsigned long long)here) - 1;
-                found = base + l;
-                *tok = (x - before - __shfl(sum - c, l, 64)) * A.tok_tile;
-                break;
-            }
-            before += __shfl(sum, 63, 64);
+// A row tile: its session, first token (of the session) and tokens, the session's
+// first row, and the first token's position.
+struct PagedTile {
+    int seq, tok, n, row0, pos0;
+};
+__device__ __forceinline__ bool paged_tile_of(const PagedDev &P, const PagedAttn &A, int seq, int tok, PagedTile *T) {
+    T->seq = uniform(seq);
+    T->tok = uniform(tok);
+    const int a = uniform(P.q_starts[T->seq]), b = uniform(P.q_starts[T->seq + 1]);
+    if (a < 0 || b > P.n_tokens || T->tok < 0 || b - a <= T->tok) return false;
+    T->n = b - a - T->tok < A.tok_tile ? b - a - T->tok : A.tok_tile;
+    T->row0 = a;
+    const int64_t pos = (int64_t)uniform(P.kv_lens[T->seq]) - (b - a) + T->tok;
+    T->pos0 = (int)(pos < -(1 << 30) ? -(1 << 30) : pos);
+    return !A.both || (b - a <= A.short_q) == (A.tok_tile == A.short_q);
+}
+// Tile x of the sessions with more than short_q rows (of all, unless both): 64
+// sessions per turn, each lane one session's tile count.
+__device__ __forceinline__ bool paged_tile(const PagedDev &P, const PagedAttn &A, int x, PagedTile *T) {
+    const int lane = threadIdx.x & 63, least = A.both ? A.short_q : 0;
+    int before = 0;
+    for (int base = 0; base < P.n_seqs; base += 64) {
+        const int i = base + lane;
+        int c = 0;
+        if (i < P.n_seqs) {
+            const int64_t len = (int64_t)P.q_starts[i + 1] - P.q_starts[i];
+            c = len > least && len <= P.n_tokens ? ((int)len + A.tok_tile - 1) / A.tok_tile : 0;
         }
-        if (found < 0) return false;
-        *seq = found;
+        int sum = c;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int up = __shfl_up(sum, o, 64);
+            if (lane >= o) sum += up;
+        }
+        const uint64_t here = __ballot(before + sum > x);
+        if (here) {
+            const int l = __ffsll((unsigned long long)here) - 1;
+            return paged_tile_of(P, A, base + l, (x - before - __shfl(sum - c, l, 64)) * A.tok_tile, T);
+        }
+        before += __shfl(sum, 63, 64);
     }
-    *seq = uniform(*seq);
-    *tok = uniform(*tok);
-    const int a = uniform(P.q_starts[*seq]), b = uniform(P.q_starts[*seq + 1]);
-    if (a < 0 || b > P.n_tokens || *tok < 0 || b - a <= *tok) return false;
-    *n = b - a - *tok < A.tok_tile ? b - a - *tok : A.tok_tile;
-    *row0 = a;
-    const int64_t pos = (int64_t)uniform(P.kv_lens[*seq]) - (b - a) + *tok;
-    *pos0 = (int)(pos < -(1 << 30) ? -(1 << 30) : pos);
-    return true;
+    return false;
 }
 
 // Cached positions [lo, hi) that any of a tile's rows attends to.
@@ -181,8 +182,9 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : G == 4 ? (R == 4 && !F32 ? 3 :
     const bool last = A.kv_mul - h0 < 16;
     const int heads = last ? A.kv_mul - h0 : 16, inv = last ? A.inv : A.inv16;
     const int split = blockIdx.y;
-    int seq, tok, n_tok, row0, pos0;
-    if (!paged_tile(P, A, tile, &seq, &tok, &n_tok, &row0, &pos0)) return;
+    PagedTile T;
+    if (!paged_tile_of(P, A, tile, 0, &T)) return;
+    const int seq = T.seq, n_tok = T.n, row0 = T.row0, pos0 = T.pos0;
     const PagedRange rg = paged_range(P, A, pos0, n_tok);
 
     // the splits' and then the waves' share of the steps
@@ -247,7 +249,7 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : G == 4 ? (R == 4 && !F32 ? 3 :
         float x[G][8], big = 0.0f;
         // a lane without a row or channel reads another's: the loads of all groups
         // are in flight together, which a branch around each would prevent
-        const int64_t from = (int64_t)(row0 + tok + (on ? my_tok : 0)) * A.q_stride +
+        const int64_t from = (int64_t)(row0 + (on ? my_tok : 0)) * A.q_stride +
                              (int64_t)(kvh * A.kv_mul + h0 + my_head) * P.hd;
 #pragma unroll
         for (int g = 0; g < G; g++) {
@@ -543,7 +545,7 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : G == 4 ? (R == 4 && !F32 ? 3 :
             sum = fmaf(f, s_l[w][r], sum);
             o = fmaf(f, s_acc[w][r][ch], o);
         }
-        const int64_t token = row0 + tok + tk;
+        const int64_t token = row0 + tk;
         if (A.n_splits > 1) {
             const int64_t to = ((int64_t)split * P.n_tokens + token) * A.n_heads + hd;
             if (top != -__builtin_inff()) A.part[to * DV + ch] = o;
@@ -569,6 +571,387 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : G == 4 ? (R == 4 && !F32 ? 3 :
     }
 }
 
+// Prompts and longer chunks: tiles of up to 128 rows (tokens x query heads of one
+// kv head), 32 per wave, whose keys and values the workgroup unpacks once per
+// 64 cached tokens into LDS: K as halves [token][channel], V as halves
+// [channel][token], times 2^E (as above, from the largest |d| of the steps so far).
+// Scores are 32x32x16 products K q^T, so that a lane holds one row's p against 16
+// tokens of each 32 and feeds them to V^T p without leaving its registers: V's
+// tokens lie in LDS in the order (quads 0 2 1 3 of 16) in which the scores come.
+// For f32 rows q, K, p and V are two halves each and the products of their small
+// parts are left out (2^-22 of the result).
+//
+// The exponentials bound it for bf16 rows: 32 scores per lane and step cost about
+// as many VALU slots as its 32 products take on the matrix cores.
+template <int G, bool F32>
+__global__ __launch_bounds__(256, G == 8 || F32 ? 1 : 2) void paged_attn_tile_kernel(PagedDev P, PagedAttn A) {
+    constexpr int DV = 32 * G, KS = DV + 8, VS = 64 + 8, N = F32 ? 2 : 1;
+    __shared__ _Float16 s_k[N][64][KS], s_v[N][DV][VS];
+    __shared__ uint32_t s_most[4], s_page[4];
+    __shared__ uint8_t s_bad[64][G];
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    const int heads_y = P.n_kv * A.n_chunk, n_tiles = (int)(gridDim.x / (uint32_t)heads_y);
+    const int x = (int)(blockIdx.x / (uint32_t)heads_y), head_y = (int)blockIdx.x - x * heads_y;
+    const int kvh = A.n_chunk == 1 ? head_y : head_y / A.n_chunk, h0 = A.n_chunk == 1 ? 0 : head_y % A.n_chunk * 16;
+    const bool last = A.kv_mul - h0 < 16;
+    const int heads = last ? A.kv_mul - h0 : 16, inv = last ? A.inv : A.inv16;
+    PagedTile T;
+    // later tiles of a prompt see more keys: they start first
+    if (!paged_tile(P, A, n_tiles - 1 - x, &T)) return;
+    const int seq = T.seq, tok = T.tok, n_tok = T.n, row0 = T.row0, pos0 = T.pos0;
+    const PagedRange rg = paged_range(P, A, pos0, n_tok);
+    const int split = blockIdx.y;
+    int per = A.split_steps;
+    if ((int64_t)per * A.n_splits < rg.steps) per = (rg.steps + A.n_splits - 1) / A.n_splits;
+    const int64_t s_at = (int64_t)split * per;
+    const int s_lo = (int)(s_at < rg.steps ? s_at : rg.steps);
+    const int s_hi = s_lo + per < rg.steps ? s_lo + per : rg.steps;
+    const int64_t head_off = (int64_t)kvh * P.block;
+
+    // a wave unpacks the 16-token tile `wave` of each step; lane j looks up where it
+    // lies in step j of the next 64
+    uint64_t where = 0, ok = 0;
+    int off_tok = 0;
+    auto look = [&](int s) __attribute__((always_inline)) {
+        const int t = rg.first + (s + lane) * 64 + 16 * wave;
+        const bool in = s + lane < s_hi && t < rg.hi;
+        int off = 0;
+        const int page = in ? paged_page(P, seq, t, &off) : -1;
+        off_tok = page < 0 ? 0 : off;
+        where = (uint64_t)(page < 0 ? 0 : page) * (uint64_t)(P.n_kv * P.block) + (uint64_t)head_off;
+        ok = __ballot(page >= 0);
+    };
+    uint32_t kr[G], vr[G], kd[G / 2], vd[2 * G];
+    bool here = false;
+    const int kt = lane >> 2, kc = lane & 3, quad = lane >> 4, vc = lane & 15;
+    auto load = [&](int s) __attribute__((always_inline)) {
+        const int l = (s - s_lo) & 63;
+        const uint64_t at = lane_u64(where, l);
+        const uint32_t off = (uint32_t)__builtin_amdgcn_readlane(off_tok, l), sc = (uint32_t)P.ps * (16 * G);
+        here = (ok >> l) & 1;
+        __builtin_memcpy(kr, P.k + at + (uint32_t)((off + kt) * (16 * G) + kc * (4 * G)), 4 * G);
+        __builtin_memcpy(kd, P.k + at + sc + (off + kt) * (2 * G), 2 * G);
+        __builtin_memcpy(vr, P.v + at + (uint32_t)(off * (16 * G) + quad * (64 * G) + vc * (4 * G)), 4 * G);
+        __builtin_memcpy(vd, P.v + at + sc + (off + 4 * quad) * (2 * G), 8 * G);
+    };
+    if (s_lo < s_hi) {
+        look(s_lo);
+        load(s_lo);
+    }
+
+    // this lane's row and its queries: B[k = 8 half + .][n = col] of each 16 channels
+    const int row = 32 * wave + col, my_tok = row * inv >> 16, my_head = row - my_tok * heads;
+    const bool on = my_tok < n_tok;
+    const int my_pos = pos0 + my_tok;
+    int rhi = on ? my_pos + 1 : 0, rlo = A.window > 0 && my_pos - A.window + 1 > 0 ? my_pos - A.window + 1 : 0;
+    if (rhi > rg.hi) rhi = rg.hi;
+    half8v q[N][2 * G];
+    float qf;
+    {
+        float v[2 * G][8], big = 0.0f;
+        const int64_t from = (int64_t)(row0 + tok + (on ? my_tok : 0)) * A.q_stride +
+                             (int64_t)(kvh * A.kv_mul + h0 + my_head) * P.hd;
+#pragma unroll
+        for (int k = 0; k < 2 * G; k++) {
+            const int ch = 16 * k + 8 * half, c = ch < P.hd ? ch : 0;
+            if (F32) {
+                row_load4((const float *)A.q + from + c, v[k]);
+                row_load4((const float *)A.q + from + c + 4, v[k] + 4);
+            } else {
+                row_load4((const uint16_t *)A.q + from + c, v[k]);
+                row_load4((const uint16_t *)A.q + from + c + 4, v[k] + 4);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 2 * G; k++) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                v[k][j] = on && 16 * k + 8 * half < P.hd ? v[k][j] : 0.0f;
+                big = fmaxf(big, fabsf(v[k][j]));
+            }
+        }
+        big = fmaxf(big, __shfl_xor(big, 32, 64));
+        int e = 0;
+        if (big > 0.0f && big < __builtin_inff()) (void)frexpf(big, &e);
+        qf = A.scale * ldexpf(1.0f, e);
+        const float down = ldexpf(1.0f, -(e >> 1)), more = ldexpf(1.0f, -(e - (e >> 1)));
+        const int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+#pragma unroll
+        for (int k = 0; k < 2 * G; k++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float y = v[k][order[j]] * down * more;
+                q[0][k][j] = (_Float16)y;
+                if (F32) q[N - 1][k][j] = (_Float16)(y - (float)q[0][k][j]);
+            }
+    }
+
+    float m = -__builtin_inff(), l = 0.0f;
+    int E = 0;
+    uint32_t limit = 0;  // the halves' bits of the largest |d| that E holds
+    f32x16v acc[G];
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[g][i] = 0.0f;
+    const int full_lo = rg.lo + (A.window > 0 ? n_tok - 1 : 0), full_hi = rg.hi - (n_tok - 1);
+    const PagedMagic magic;
+
+    for (int s = s_lo; s < s_hi; s++) {
+        const int t0 = rg.first + s * 64;
+        // scales of tokens that no row sees become 0; the largest of the others
+        const bool all = t0 + 16 * wave >= rg.lo && t0 + 16 * wave + 16 <= rg.hi && here;
+        if (!all) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int t = t0 + 16 * wave + 4 * quad + r;
+                const bool out = t < rg.lo || t >= rg.hi || !here;
+#pragma unroll
+                for (int g = 0; g < G; g++) {
+                    const int e = r * G + g;
+                    vd[e >> 1] &= out ? (e & 1 ? 0x0000FFFFu : 0xFFFF0000u) : 0xFFFFFFFFu;
+                }
+            }
+        }
+        uint32_t most = 0;
+#pragma unroll
+        for (int j = 0; j < 2 * G; j++) {
+            const uint32_t a = vd[j] & 0x7FFFu, b = (vd[j] >> 16) & 0x7FFFu;
+            most = most > a ? most : a;
+            most = most > b ? most : b;
+        }
+        if (__ballot(most > limit)) {
+            for (int o = 32; o > 0; o >>= 1) {
+                const uint32_t y = (uint32_t)__shfl_xor((int)most, o, 64);
+                most = most > y ? most : y;
+            }
+        }
+        if (lane == 0) s_most[wave] = most;
+        __syncthreads();  // and every wave has read the step before
+        uint32_t top = s_most[0];
+#pragma unroll
+        for (int w = 1; w < 4; w++) top = top > s_most[w] ? top : s_most[w];
+        top = (uint32_t)uniform((int)top);
+        bool bad = false;
+        if (top > limit) {
+            bad = top >= 0x7C00u;  // NaN or infinity among them
+            if (bad) {
+                // those groups become 0 here and NaN to the rows that see them
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int g = 0; g < G; g++) {
+                        const int e = r * G + g;
+                        const uint32_t w = (vd[e >> 1] >> (16 * (e & 1))) & 0x7FFFu;
+                        if (vc == 0) s_bad[16 * wave + 4 * quad + r][g] = w >= 0x7C00u;
+                        if (w >= 0x7C00u) vd[e >> 1] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                    }
+                top = 0x7BFFu;
+            }
+            if (top > limit) {
+                // |d| < 2^e, d 2^E <= 2^12, |d (c - 8)| 2^E <= 2^15
+                int e;
+                (void)frexpf(h2f((uint16_t)top), &e);
+                const int was = E;
+                E = 12 - e;
+                limit = 0x7BFFu;
+                if (e < 15) limit = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)ldexpf(1.0f, e));
+                if (m != -__builtin_inff()) {
+                    const float a = ldexpf(1.0f, E - was);
+#pragma unroll
+                    for (int g = 0; g < G; g++) acc[g] *= a;
+                }
+            }
+        }
+        // unpack: keys of token kt, channels 32 g + 8 kc ..; values of quad `quad`,
+        // channels 32 g + vc and 32 g + 16 + vc
+        {
+            const int t = 16 * wave + kt;
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                const _Float16 d = paged_h2(kd[g >> 1])[g & 1];
+                const half2v d2 = {d, d};
+                // in the order 0 4 1 5 2 6 3 7 of each eight channels, as the queries
+                const u32x4v c = __builtin_bit_cast(u32x4v, magic.k8(kr[g]));
+                u32x4v hi, lo;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t cj = c[j];
+                    const half2v p = paged_h2(cj) * d2;
+                    hi[j] = __builtin_bit_cast(uint32_t, p);
+                    if (F32) {
+                        half2v r;
+#pragma unroll
+                        for (int y = 0; y < 2; y++) r[y] = (_Float16)fmaf((float)paged_h2(cj)[y], (float)d, -(float)p[y]);
+                        lo[j] = __builtin_bit_cast(uint32_t, r);
+                    }
+                }
+                *(u32x4v *)&s_k[0][t][32 * g + 8 * kc] = hi;
+                if (F32) *(u32x4v *)&s_k[N - 1][t][32 * g + 8 * kc] = lo;
+            }
+            const int at = 16 * wave + 4 * (2 * (quad & 1) + (quad >> 1));
+            const float up = ldexpf(1.0f, E);
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                uint32_t hi[2][2], lo[2][2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int b0 = 2 * h * G + g, b1 = (2 * h + 1) * G + g;
+                    const uint32_t w = __builtin_amdgcn_perm(vr[b1 >> 2], vr[b0 >> 2],
+                                                             0x0C000C00u | (uint32_t)(b0 & 3) |
+                                                                 (uint32_t)(4 + (b1 & 3)) << 16);
+                    // d 2^E as a float (the half may be subnormal), exact as a half
+                    const float d0 = (float)paged_h2(vd[b0 >> 1])[b0 & 1] * up;
+                    const float d1 = (float)paged_h2(vd[b1 >> 1])[b1 & 1] * up;
+                    const half2v dd = {(_Float16)d0, (_Float16)d1};
+                    const uint32_t cw[2] = {magic.low(w), magic.high(w)};
+#pragma unroll
+                    for (int n = 0; n < 2; n++) {
+                        const half2v c = paged_h2(cw[n]), y = c * dd;
+                        hi[n][h] = __builtin_bit_cast(uint32_t, y);
+                        if (F32) {
+                            half2v r;
+                            r[0] = (_Float16)fmaf((float)c[0], (float)dd[0], -(float)y[0]);
+                            r[1] = (_Float16)fmaf((float)c[1], (float)dd[1], -(float)y[1]);
+                            lo[n][h] = __builtin_bit_cast(uint32_t, r);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    *(uint2 *)&s_v[0][32 * g + 16 * n + vc][at] = make_uint2(hi[n][0], hi[n][1]);
+                    if (F32) *(uint2 *)&s_v[N - 1][32 * g + 16 * n + vc][at] = make_uint2(lo[n][0], lo[n][1]);
+                }
+            }
+        }
+        if (lane == 0) s_page[wave] = here;
+        if (((s + 1 - s_lo) & 63) == 0 && s + 1 < s_hi) look(s + 1);
+        load(s + 1 < s_hi ? s + 1 : s);
+        __syncthreads();
+
+        bool pages[4];
+#pragma unroll
+        for (int w = 0; w < 4; w++) pages[w] = uniform((int)s_page[w]) != 0;
+        const bool full = t0 >= full_lo && t0 + 64 <= full_hi && pages[0] && pages[1] && pages[2] && pages[3];
+        // scores of 64 tokens: [32-token tile][16]
+        f32x16v sc[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) sc[u][i] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 2 * G; k++) {
+                const half8v a = *(const half8v *)&s_k[0][32 * u + col][16 * k + 8 * half];
+                sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[0][k], sc[u], 0, 0, 0);
+                if (F32) {
+                    const half8v b = *(const half8v *)&s_k[N - 1][32 * u + col][16 * k + 8 * half];
+                    sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[N - 1][k], sc[u], 0, 0, 0);
+                    sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, q[0][k], sc[u], 0, 0, 0);
+                }
+            }
+        }
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                sc[u][i] *= qf;
+                if (!full) {
+                    const int k = 32 * u + 8 * (i >> 2) + 4 * half + (i & 3), t = t0 + k;
+                    const bool page = pages[2 * u + (i >> 3)];
+                    if (t < rlo || t >= rhi || !page) sc[u][i] = -__builtin_inff();
+                }
+                mx = fmaxf(mx, sc[u][i]);
+            }
+        // m follows the maximum only when it is 8 behind: p 2^6 stays at or below 2^14,
+        // and keeps all its bits as a half down to 2^-28 of that
+        if (__ballot(mx > m + 8.0f || (m == -__builtin_inff() && mx > m))) {
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            mx = fmaxf(mx, m);
+            const float a = m == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
+            m = mx;
+            l *= a;
+#pragma unroll
+            for (int g = 0; g < G; g++) acc[g] *= a;
+        }
+        const float base = (m == -__builtin_inff() ? 0.0f : m) - 6.0f;
+        half8v ph[4], pl[F32 ? 4 : 1];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float p = __builtin_amdgcn_exp2f(sc[u][i] - base);
+                l += p;
+                ph[2 * u + (i >> 3)][i & 7] = (_Float16)p;
+                if (F32) pl[F32 ? 2 * u + (i >> 3) : 0][i & 7] = (_Float16)(p - (float)(_Float16)p);
+            }
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const half8v a = *(const half8v *)&s_v[0][32 * g + col][16 * c + 8 * half];
+                acc[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[c], acc[g], 0, 0, 0);
+                if (F32) {
+                    const half8v b = *(const half8v *)&s_v[N - 1][32 * g + col][16 * c + 8 * half];
+                    acc[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[F32 ? c : 0], acc[g], 0, 0, 0);
+                    acc[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, ph[c], acc[g], 0, 0, 0);
+                }
+            }
+        if (bad) {
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                bool sees = false;
+                for (int k = 0; k < 64; k++) sees |= s_bad[k][g] && t0 + k >= rlo && t0 + k < rhi;
+                if (sees) acc[g] += __builtin_nanf("");
+            }
+        }
+    }
+
+    l += __shfl_xor(l, 32, 64);
+    l *= 1.0f / 64.0f;
+    if (!on) return;
+    const float unit = ldexpf(1.0f, -E - 6);
+    const int hd = kvh * A.kv_mul + h0 + my_head;
+    const int64_t token = row0 + tok + my_tok;
+    const bool none = m == -__builtin_inff();
+    if (A.n_splits > 1) {
+        const int64_t to = ((int64_t)split * P.n_tokens + token) * A.n_heads + hd;
+        if (half == 0) {
+            A.ml[to * 2] = m;
+            A.ml[to * 2 + 1] = l;
+        }
+        if (!none)
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const float y[4] = {acc[g][i] * unit, acc[g][i + 1] * unit, acc[g][i + 2] * unit, acc[g][i + 3] * unit};
+                    row_store4(A.part + to * DV + 32 * g + 2 * i + 4 * half, y);
+                }
+        return;
+    }
+    float f = none ? 0.0f : unit / l;
+    if (A.sinks && !none) {
+        const float sink = A.sinks[hd] * 1.44269504f, top = fmaxf(m, sink), a = __builtin_amdgcn_exp2f(m - top);
+        f = unit * a / fmaf(l, a, __builtin_amdgcn_exp2f(sink - top));
+    }
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int ch = 32 * g + 2 * i + 4 * half;
+            if (ch >= P.vd) continue;
+            const float y[4] = {none ? 0.0f : acc[g][i] * f, none ? 0.0f : acc[g][i + 1] * f,
+                                none ? 0.0f : acc[g][i + 2] * f, none ? 0.0f : acc[g][i + 3] * f};
+            const int64_t to = token * A.o_stride + (int64_t)hd * P.vd + ch;
+            if (F32)
+                row_store4((float *)A.out + to, y);
+            else
+                row_store4((uint16_t *)A.out + to, y);
+        }
+}
+
 // Joins a row's splits.  One workgroup per (token, query head): the splits'
 // weights first, then each of 256 / DV groups of threads sums every so-manieth
 // split, eight loads in flight, and the groups' sums are added in their order.
@@ -578,15 +961,21 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedDev P, PagedA
     __shared__ float s_f[256], s_o[N][DV], s_red[4];
     const int64_t rows = (int64_t)P.n_tokens * A.n_heads, w = blockIdx.x;
     const int token = (int)(w / A.n_heads), hd = (int)(w % A.n_heads);
-    const int i = threadIdx.x;  // n_splits <= 256
+    const int i = threadIdx.x;  // at most 256 splits
+    const int most = A.n_splits > A.tile_splits ? A.n_splits : A.tile_splits;
     float m = -__builtin_inff(), part = 0.0f;
-    if (i < A.n_splits) {
+    if (i < most) {
         m = A.ml[(i * rows + w) * 2];
         part = A.ml[(i * rows + w) * 2 + 1];
     }
     int seq, a, b;
-    // rows of no tile stay as they are
-    if (!paged_session(P, token, &seq, &a, &b) || (A.by_seq && token - a >= A.tok_tile)) return;
+    // rows of no tile stay as they are, rows of one split are done
+    if (!paged_session(P, token, &seq, &a, &b)) return;
+    const bool tiled = A.short_q == 0 || (A.both && b - a > A.short_q);
+    if (!tiled && token - a >= A.short_q) return;
+    const int n_splits = tiled ? A.tile_splits : A.n_splits;
+    if (n_splits <= 1) return;
+    if (i >= n_splits) m = -__builtin_inff();
     const float top = block_max_256(m, s_red);
     const bool none = top == -__builtin_inff();
     float base = none ? 0.0f : top, sink = 0.0f;
@@ -600,12 +989,12 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedDev P, PagedA
     const float sum = block_sum_256(f == 0.0f ? 0.0f : f * part, s_red) + sink;  // the barriers order s_f too
     const int ch = i % DV;
     float o[4] = {0, 0, 0, 0};
-    for (int s = i / DV; s < A.n_splits; s += 8 * N) {
+    for (int s = i / DV; s < n_splits; s += 8 * N) {
         float x[8], f8[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const int at = s + j * N < A.n_splits ? s + j * N : 0;
-            f8[j] = s + j * N < A.n_splits ? s_f[at] : 0.0f;
+            const int at = s + j * N < n_splits ? s + j * N : 0;
+            f8[j] = s + j * N < n_splits ? s_f[at] : 0.0f;
             x[j] = A.part[(at * rows + w) * DV + ch];
         }
 #pragma unroll

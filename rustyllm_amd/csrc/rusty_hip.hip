@@ -4468,45 +4468,64 @@ struct PagedDevice {
     }
 };
 
-// How a call's attention is cut: rows per tile, waves per tile, and splits of a
-// tile's cached range.
+// How a call's attention is cut.  Sessions of few rows (R of tokens x query heads of
+// a kv head) are a row tile each; the others are tiles of 128 rows.
 struct PagedPlan {
-    int R, W, tok_tile, by_seq, n_splits, split_steps;
-    int64_t tiles, heads_y;
+    int R = 0, W = 0, short_q = 0, splits = 1, steps = 0;  // row tiles, short_q = 0: none
+    int tok_tile = 0, tile_splits = 1, tile_steps = 0;     // 128-row tiles, tok_tile = 0: none
+    int64_t tiles = 0, heads_y = 0;
 };
 static PagedPlan paged_plan(const PagedDev &P, uint32_t n_heads, uint32_t max_q, uint32_t max_kv, uint32_t window) {
     PagedPlan p;
     const int kv_mul = (int)n_heads / P.n_kv, chunk = kv_mul < 16 ? kv_mul : 16;
-    const bool wide = P.hd > 128 || P.vd > 128;  // 4-row tiles there would not fit the registers
-    const int64_t rows = (int64_t)chunk * (max_q < 16 ? max_q : 16);
-    p.R = rows <= 4 && !wide ? 4 : rows <= 8 ? 8 : 16;
-    p.tok_tile = p.R / chunk;
-    p.by_seq = max_q <= (uint32_t)p.tok_tile;
-    p.tiles = p.by_seq ? P.n_seqs : P.n_tokens / p.tok_tile + (int64_t)P.n_seqs;
+    const int least = P.hd > 128 || P.vd > 128 ? 8 : 4;  // 4-row tiles of wide heads would not fit the registers
     p.heads_y = (int64_t)P.n_kv * ((kv_mul + 15) / 16);
-    int64_t seen = max_kv;
-    if (window && (int64_t)window + p.tok_tile + 15 < seen) seen = (int64_t)window + p.tok_tile + 15;
-    const int64_t steps = seen > 0 ? (seen + 63) / 64 : 1, items = p.tiles * p.heads_y;
-    // Eight waves per CU or more of short (tile, kv head) pairs: a wave each (256
-    // sessions of 128 positions, 8 kv heads: 15.0 us, 16.8 with a workgroup each).
-    // Otherwise a workgroup each, and splits of 4 to 64 steps (1 to 16 per wave) for
-    // three workgroups per CU: 48 ragged sessions of up to 8192 take 76 us with 64
-    // steps, 80 with 16; one of 131072 takes 36 and 43.
-    p.W = items >= 2048 && steps <= 16 ? 1 : 4;
-    int64_t per = 16;
-    if (p.W == 4) {
-        per = (steps * items + 767) / 768;
-        per = per < 4 ? 4 : per > 64 ? 64 : per;
+    auto steps_of = [&](int64_t tokens) {
+        int64_t seen = max_kv;
+        if (window && (int64_t)window + tokens + 15 < seen) seen = (int64_t)window + tokens + 15;
+        return seen > 0 ? (seen + 63) / 64 : 1;
+    };
+    const bool tiles = (int64_t)max_q * chunk > 16;
+    // rows a session may have as a row tile; where all have max_q rows there is none
+    const int64_t rows = tiles ? chunk : (int64_t)max_q * chunk;
+    if (!tiles || (uint64_t)P.n_seqs * max_q != (uint64_t)P.n_tokens) {
+        p.R = rows <= least ? least : rows <= 8 ? 8 : 16;
+        p.short_q = p.R / chunk;
+        const int64_t steps = steps_of(p.short_q), items = P.n_seqs * p.heads_y;
+        // Eight waves per CU or more of short (tile, kv head) pairs: a wave each (256
+        // sessions of 128 positions, 8 kv heads: 15.0 us, 16.8 with a workgroup each).
+        // Otherwise a workgroup each, and splits of 4 to 64 steps (1 to 16 per wave) for
+        // three workgroups per CU: 48 ragged sessions of up to 8192 take 76 us with 64
+        // steps, 80 with 16; one of 131072 takes 36 and 43.
+        p.W = items >= 2048 && steps <= 16 ? 1 : 4;
+        int64_t per = 16;
+        if (p.W == 4) {
+            per = (steps * items + 767) / 768;
+            per = per < 4 ? 4 : per > 64 ? 64 : per;
+        }
+        if (steps <= per + per / 2) per = steps;
+        if ((steps + per - 1) / per > 256) per = (steps + 255) / 256;
+        p.splits = (int)((steps + per - 1) / per);
+        p.steps = (int)per;
     }
-    if (steps <= per + per / 2) per = steps;
-    if ((steps + per - 1) / per > 256) per = (steps + 255) / 256;
-    p.n_splits = (int)((steps + per - 1) / per);
-    p.split_steps = (int)per;
+    if (tiles) {
+        p.tok_tile = 128 / chunk;
+        p.tiles = P.n_tokens / p.tok_tile + (int64_t)P.n_seqs;
+        // two workgroups per CU, of 4 steps or more each
+        const int64_t steps = steps_of(p.tok_tile), items = (P.n_tokens + p.tok_tile - 1) / p.tok_tile * p.heads_y;
+        int64_t n = 512 / items;
+        if (n > (steps + 3) / 4) n = (steps + 3) / 4;
+        if (n < 1) n = 1;
+        if (n > 256) n = 256;
+        p.tile_splits = (int)n;
+        p.tile_steps = (int)((steps + n - 1) / n);
+    }
     return p;
 }
 static uint64_t paged_workspace(const PagedDev &P, const PagedPlan &p, uint32_t n_heads) {
-    if (p.n_splits <= 1) return 0;
-    return (uint64_t)p.n_splits * P.n_tokens * n_heads * (32 * paged_groups(P.hd, P.vd) + 2) * 4;
+    const int n = p.splits > p.tile_splits ? p.splits : p.tile_splits;
+    if (n <= 1) return 0;
+    return (uint64_t)n * P.n_tokens * n_heads * (32 * paged_groups(P.hd, P.vd) + 2) * 4;
 }
 static bool paged_heads_ok(const PagedDev &P, uint32_t n_heads) {
     return n_heads && n_heads <= 65536 && n_heads % P.n_kv == 0;
@@ -4514,7 +4533,7 @@ static bool paged_heads_ok(const PagedDev &P, uint32_t n_heads) {
 
 template <int G, bool F32, int W>
 static void paged_attn_rows_launch(const PagedDev &P, const PagedAttn &A, const PagedPlan &p, hipStream_t s) {
-    const dim3 grid((unsigned)(p.tiles * p.heads_y), (unsigned)p.n_splits);
+    const dim3 grid((unsigned)(P.n_seqs * p.heads_y), (unsigned)p.splits);
     if (p.R == 16)
         paged_attn_rows_kernel<G, 16, F32, W><<<grid, 64 * W, 0, s>>>(P, A);
     else if (p.R == 8)
@@ -4523,13 +4542,31 @@ static void paged_attn_rows_launch(const PagedDev &P, const PagedAttn &A, const 
         paged_attn_rows_kernel<G, 4, F32, W><<<grid, 64 * W, 0, s>>>(P, A);
 }
 template <int G, bool F32>
-static void paged_attn_launch(const PagedDev &P, const PagedAttn &A, const PagedPlan &p, hipStream_t s) {
-    if (p.W == 1)
-        paged_attn_rows_launch<G, F32, 1>(P, A, p, s);
-    else
-        paged_attn_rows_launch<G, F32, 4>(P, A, p, s);
-    if (p.n_splits > 1)
+static void paged_attn_launch(const PagedDev &P, PagedAttn A, const PagedPlan &p, hipStream_t s) {
+    const int last = A.kv_mul & 15;  // query heads of a kv head's last sixteen
+    auto tiles_of = [&](int tokens, int splits, int steps, int unit) {
+        A.tok_tile = tokens;
+        A.n_splits = splits;
+        A.split_steps = steps;
+        A.inv16 = unit / 16;
+        A.inv = last ? (unit + last - 1) / last : unit / 16;
+    };
+    if (p.tok_tile) {
+        tiles_of(p.tok_tile, p.tile_splits, p.tile_steps, 1 << 16);
+        const dim3 grid((unsigned)(p.tiles * p.heads_y), (unsigned)p.tile_splits);
+        paged_attn_tile_kernel<G, F32><<<grid, 256, 0, s>>>(P, A);
+    }
+    if (p.short_q) {
+        tiles_of(p.short_q, p.splits, p.steps, 1 << 8);
+        if (p.W == 1)
+            paged_attn_rows_launch<G, F32, 1>(P, A, p, s);
+        else
+            paged_attn_rows_launch<G, F32, 4>(P, A, p, s);
+    }
+    if (p.splits > 1 || p.tile_splits > 1) {
+        A.n_splits = p.splits;
         paged_attn_join_kernel<G, F32><<<(unsigned)((int64_t)P.n_tokens * A.n_heads), 256, 0, s>>>(P, A);
+    }
 }
 
 }  // namespace rh
@@ -4669,26 +4706,24 @@ int rusty_hip_paged_attention(const RustyPagedKv *kv, const RustyPagedBatch *bat
     const PagedPlan p = paged_plan(P, rows->n_heads, batch->max_q_len, batch->max_kv_len, rows->window);
     const uint64_t need = paged_workspace(P, p, rows->n_heads);
     if (need && (!rows->workspace || rows->workspace_len < need || (uintptr_t)rows->workspace % 16)) return 0;
-    if (p.tiles * p.heads_y > (0x7FFFFFFF >> 8) || (int64_t)n * rows->n_heads > 0x7FFFFFFF) return 0;
+    if (p.tiles * p.heads_y > (0x7FFFFFFF >> 8) || P.n_seqs * p.heads_y > (0x7FFFFFFF >> 8) || (int64_t)n * rows->n_heads > 0x7FFFFFFF) return 0;
     PagedAttn A;
     A.q = rows->q;
     A.out = rows->out;
     A.sinks = rows->sinks;
     A.part = need ? (float *)rows->workspace : nullptr;
-    A.ml = need ? A.part + (int64_t)p.n_splits * P.n_tokens * rows->n_heads * 32 * paged_groups(P.hd, P.vd) : nullptr;
+    const int64_t splits = p.splits > p.tile_splits ? p.splits : p.tile_splits;
+    A.ml = need ? A.part + splits * P.n_tokens * rows->n_heads * 32 * paged_groups(P.hd, P.vd) : nullptr;
     A.q_stride = rows->q_stride;
     A.o_stride = rows->out_stride;
     A.scale = rows->scale * 1.44269504f;
     A.n_heads = (int)rows->n_heads;
     A.kv_mul = (int)rows->n_heads / P.n_kv;
     A.n_chunk = (A.kv_mul + 15) / 16;
-    A.inv16 = 16;
-    A.inv = (A.kv_mul & 15) ? (256 + (A.kv_mul & 15) - 1) / (A.kv_mul & 15) : 16;
     A.window = (int)rows->window;
-    A.tok_tile = p.tok_tile;
-    A.n_splits = p.n_splits;
-    A.split_steps = p.split_steps;
-    A.by_seq = p.by_seq;
+    A.short_q = p.short_q;
+    A.both = p.short_q && p.tok_tile;
+    A.tile_splits = p.tile_splits;
     hipStream_t s = (hipStream_t)stream;
     const int G = paged_groups(P.hd, P.vd);
     if (rows->dtype)

@@ -66,15 +66,8 @@ class Pool:
 
     def load(self, which, page, off):
         """[n_kv][dim] values (f64, exact)."""
-        return self._load(which, page, off)[0]
-
-    def scales(self, which, page, off):
-        """[n_kv][dim] magnitudes of the values' steps."""
-        return self._load(which, page, off)[1]
-
-    def _load(self, which, page, off):
         buf, G = (self.k if which == "k" else self.v), self.G
-        out, step = np.zeros((self.n_kv, 32 * G)), np.zeros((self.n_kv, 32 * G))
+        out = np.zeros((self.n_kv, 32 * G))
         for h in range(self.n_kv):
             at = self._at(page, h)
             for g in range(G):
@@ -89,9 +82,7 @@ class Pool:
                     b = buf[first:first + 64 * G:4 * G][:16]
                     c[:16], c[16:] = b & 15, b >> 4
                 out[h, 32 * g:32 * g + 32] = d * (c - 8)
-                step[h, 32 * g:32 * g + 32] = abs(d)
-        dim = self.hd if which == "k" else self.vd
-        return out[:, :dim], step[:, :dim]
+        return out[:, :self.hd if which == "k" else self.vd]
 
 
 def rotate(x, cos, sin, neox):
@@ -112,14 +103,14 @@ def rotate(x, cos, sin, neox):
 
 def attention(pool, table, kv_lens, q_starts, q, scale, window=0, sinks=None):
     """64-bit attention of q [rows][heads][hd].  Returns out, and per (row, head)
-    the bounds that a tolerance is made of: sum p |v| / sum p and sum p |d| / sum p
-    per channel (stacked), and max |q| sum |k|, sum |q k| at their largest over the
-    row's keys."""
+    the bounds that a tolerance is made of: sum p |v| / sum p per channel, and of
+    scale times the row's keys at their largest 2 max |q| sum |k| + hd sum |q k|, and
+    sum |q k|."""
     rows, heads, hd = q.shape
     mul = heads // pool.n_kv
     out = np.full((rows, heads, pool.vd), np.nan)
-    spread = np.zeros((2, rows, heads, pool.vd))
-    size = np.zeros((rows, heads))
+    spread = np.zeros((rows, heads, pool.vd))
+    size = np.zeros((2, rows, heads))
     cached = {}
     for s in range(len(kv_lens)):
         a, b = q_starts[s], q_starts[s + 1]
@@ -137,10 +128,9 @@ def attention(pool, table, kv_lens, q_starts, q, scale, window=0, sinks=None):
                 continue
             for key in keys:
                 if key not in cached:
-                    cached[key] = (pool.load("k", *key), pool.load("v", *key), pool.scales("v", *key))
+                    cached[key] = (pool.load("k", *key), pool.load("v", *key))
             k = np.stack([cached[key][0] for key in keys])
             v = np.stack([cached[key][1] for key in keys])
-            d = np.stack([cached[key][2] for key in keys])
             for h in range(heads):
                 x = q[r, h].astype(np.float64)
                 w = scale * (k[:, h // mul] @ x)
@@ -148,29 +138,28 @@ def attention(pool, table, kv_lens, q_starts, q, scale, window=0, sinks=None):
                 p = np.exp(w - top)
                 total = p.sum() + (0.0 if sinks is None else np.exp(float(sinks[h]) - top))
                 out[r, h] = p @ v[:, h // mul] / total
-                spread[0, r, h] = p @ np.abs(v[:, h // mul]) / total
-                spread[1, r, h] = p @ d[:, h // mul] / total
+                spread[r, h] = p @ np.abs(v[:, h // mul]) / total
                 ka = np.abs(k[:, h // mul])
-                size[r, h] = abs(scale) * (2 * np.abs(x).max() * ka.sum(1).max() + hd * (ka @ np.abs(x)).max())
+                size[1, r, h] = abs(scale) * (ka @ np.abs(x)).max()
+                size[0, r, h] = abs(scale) * 2 * np.abs(x).max() * ka.sum(1).max() + hd * size[1, r, h]
     return out, spread, size
 
 
 def tolerance(out, spread, size, dtype):
     """How far a computed value may be from the 64-bit one.
 
-    Scores: a query is held to 2^-24 of its row's largest value, the codes and
-    scales are exact, and at most hd + 8 f32 additions and multiplications round
-    by 2^-24 each of partial sums no larger than sum |q k|: together under
-    2^-24 * 2 * size.  A score off by x changes p by a factor within exp(+-x), in
-    the numerator and in the sum: 2 x (1.1 for the second order; x < 0.05).  exp2
-    itself and the running rescales: 2^-19.  p d is held to 2^-17 (two bf16 terms,
-    f32 rows) or 2^-8 (bf16 rows), of each term's magnitude.  The f32 sums over
-    the cached rows: 2^-17.  A product of 32 rows adds p d (128 + c) to -136 sum p d,
-    so two f32 results (four for f32 rows, whose second terms are 2^-8 of the
-    first) of up to 136 sum p d round by 2^-23 each: 2 (1 + 2^-8) 136 2^-23 < 2^-14.9
-    of sum p d.  bf16 outputs round by 2^-8 of themselves."""
-    x = 2.0 ** -23 * size
+    Scores: a query is held to 2^-24 of its row's largest value, codes and scales
+    are exact, and at most hd + 8 f32 additions and multiplications round by 2^-24
+    each of partial sums no larger than sum |q k|: together under 2^-23 size[0].  In
+    a long chunk's bf16 rows a key is one half besides: 2^-12 size[1].  A score off
+    by x changes p by a factor within exp(+-x), in the numerator and in the sum: 2 x
+    (1.1 for the second order; x < 0.05).  exp2 itself and the running rescales:
+    2^-19.  p d, or p and d (c - 8), are two halves each for f32 rows, less the
+    product of the small ones: 2^-20 of each term; one half each for bf16 rows:
+    2^-11.  The f32 sums over the cached rows: 2^-17.  bf16 outputs round by 2^-8 of
+    themselves."""
+    x = 2.0 ** -23 * size[0] + (2.0 ** -12 * size[1] if dtype == "bf16" else 0.0)
     assert x.max(initial=0.0) < 0.05
-    rel = 2.2 * x + 2.0 ** -19 + 2.0 ** -17 + (2.0 ** -17 if dtype == "f32" else 2.0 ** -8)
-    tol = spread[0] * rel[..., None] + spread[1] * 2.0 ** -14.9 + 1e-30
+    rel = 2.2 * x + 2.0 ** -19 + 2.0 ** -17 + (2.0 ** -20 if dtype == "f32" else 2.0 ** -11)
+    tol = spread * rel[..., None] + 1e-30
     return tol + (2.0 ** -8 * (np.abs(out) + tol) if dtype == "bf16" else 0.0)
