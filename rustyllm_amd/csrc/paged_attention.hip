@@ -29,7 +29,6 @@ struct PagedAttn {
     int32_t split_steps; // 64-token steps of a split, more where n_splits would not cover the range
     int32_t short_q;     // sessions of up to so many rows are row tiles of their own (paged_attn_rows_kernel)
     int32_t both;        // 1: the others are paged_attn_tile_kernel's; 0: all are of one kind
-    int32_t tile_splits; // n_splits of the others (for the join)
 };
 
 // A row tile: its session, first token (of the session) and tokens, the session's
@@ -571,25 +570,37 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : G == 4 ? (R == 4 && !F32 ? 3 :
     }
 }
 
-// Prompts and longer chunks: tiles of up to 128 rows (tokens x query heads of one
+// Prompts and longer chunks: tiles of up to 32 W rows (tokens x query heads of one
 // kv head), 32 per wave, whose keys and values the workgroup unpacks once per
 // 64 cached tokens into LDS: K as halves [token][channel], V as halves
-// [channel][token], times 2^E (as above, from the largest |d| of the steps so far).
-// Scores are 32x32x16 products K q^T, so that a lane holds one row's p against 16
-// tokens of each 32 and feeds them to V^T p without leaving its registers: V's
-// tokens lie in LDS in the order (quads 0 2 1 3 of 16) in which the scores come.
+// [channel][token] times 2^E, where E keeps the largest |d| of the steps so far at
+// 2^12.  Of 8 waves four unpack keys and four values, of 4 each does both.  Scores
+// are 32x32x16 products K q^T, so that a lane holds one row's p against 16 tokens of
+// each 32 and feeds them to V^T p without leaving its registers: V's tokens lie in
+// LDS in the order (quads 0 2 1 3 of 16) in which the scores come.  LDS holds two
+// steps: one is unpacked while the other is worked on, with one barrier per step.
 // For f32 rows q, K, p and V are two halves each and the products of their small
 // parts are left out (2^-22 of the result).
 //
-// The exponentials bound it for bf16 rows: 32 scores per lane and step cost about
-// as many VALU slots as its 32 products take on the matrix cores.
-template <int G, bool F32>
-__global__ __launch_bounds__(256, G == 8 || F32 ? 1 : 2) void paged_attn_tile_kernel(PagedDev P, PagedAttn A) {
-    constexpr int DV = 32 * G, KS = DV + 8, VS = 64 + 8, N = F32 ? 2 : 1;
-    __shared__ _Float16 s_k[N][64][KS], s_v[N][DV][VS];
-    __shared__ uint32_t s_most[4], s_page[4];
-    __shared__ uint8_t s_bad[64][G];
-    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+// VALU issue bounds it for bf16 rows: a wave's 32 x 64 scores cost about 150
+// instructions (32 of them exponentials at a quarter of the rate), its share of the
+// unpacking 75, against 32 products of 32 clocks.
+template <int G, bool F32, int W>
+__global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void paged_attn_tile_kernel(PagedDev P, PagedAttn A) {
+    constexpr int DV = 32 * G, N = F32 ? 2 : 1, NB = G == 8 && F32 ? 1 : 2, SETS = W == 8 ? 1 : 2;
+    __shared__ half8v s_k[NB][N][64 * DV / 8], s_v[NB][N][DV * 64 / 8];
+    __shared__ uint32_t s_most[2][4], s_page[2][4];
+    __shared__ uint8_t s_bad[2][64][G];
+    // Row r's 16-byte piece c lies at r * pieces + (c ^ h(r)): the 16 rows that a
+    // quarter wave reads at one c, and the 4 x 4 (row, piece) it writes, fall on
+    // different banks.
+    auto k_at = [](int r, int c) __attribute__((always_inline)) {
+        const int h = G == 2 ? ((r >> 1) & 1) << 2 | ((r >> 2) & 3) : (r & 3) << 2 | ((r >> 2) & 3);
+        return r * (DV / 8) + (c ^ h);
+    };
+    auto v_at = [](int r, int c) __attribute__((always_inline)) { return r * 8 + (c ^ ((r >> 1) & 7)); };
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), w4 = wave & 3;
+    const bool do_k = W == 4 || wave < 4, do_v = W == 4 || wave >= 4;
     const int col = lane & 31, half = lane >> 5;
     const int heads_y = P.n_kv * A.n_chunk, n_tiles = (int)(gridDim.x / (uint32_t)heads_y);
     const int x = (int)(blockIdx.x / (uint32_t)heads_y), head_y = (int)blockIdx.x - x * heads_y;
@@ -609,12 +620,12 @@ __global__ __launch_bounds__(256, G == 8 || F32 ? 1 : 2) void paged_attn_tile_ke
     const int s_hi = s_lo + per < rg.steps ? s_lo + per : rg.steps;
     const int64_t head_off = (int64_t)kvh * P.block;
 
-    // a wave unpacks the 16-token tile `wave` of each step; lane j looks up where it
-    // lies in step j of the next 64
+    // a wave unpacks the 16-token tile w4 of each step; lane j looks up where it lies
+    // in step j of the next 64
     uint64_t where = 0, ok = 0;
     int off_tok = 0;
     auto look = [&](int s) __attribute__((always_inline)) {
-        const int t = rg.first + (s + lane) * 64 + 16 * wave;
+        const int t = rg.first + (s + lane) * 64 + 16 * w4;
         const bool in = s + lane < s_hi && t < rg.hi;
         int off = 0;
         const int page = in ? paged_page(P, seq, t, &off) : -1;
@@ -622,7 +633,7 @@ __global__ __launch_bounds__(256, G == 8 || F32 ? 1 : 2) void paged_attn_tile_ke
         where = (uint64_t)(page < 0 ? 0 : page) * (uint64_t)(P.n_kv * P.block) + (uint64_t)head_off;
         ok = __ballot(page >= 0);
     };
-    uint32_t kr[G], vr[G], kd[G / 2], vd[2 * G];
+    uint32_t code[SETS][G], scale[SETS][2 * G];  // a step as it is stored: keys in set 0, values in the last
     bool here = false;
     const int kt = lane >> 2, kc = lane & 3, quad = lane >> 4, vc = lane & 15;
     auto load = [&](int s) __attribute__((always_inline)) {
@@ -630,10 +641,22 @@ __global__ __launch_bounds__(256, G == 8 || F32 ? 1 : 2) void paged_attn_tile_ke
         const uint64_t at = lane_u64(where, l);
         const uint32_t off = (uint32_t)__builtin_amdgcn_readlane(off_tok, l), sc = (uint32_t)P.ps * (16 * G);
         here = (ok >> l) & 1;
-        __builtin_memcpy(kr, P.k + at + (uint32_t)((off + kt) * (16 * G) + kc * (4 * G)), 4 * G);
-        __builtin_memcpy(kd, P.k + at + sc + (off + kt) * (2 * G), 2 * G);
-        __builtin_memcpy(vr, P.v + at + (uint32_t)(off * (16 * G) + quad * (64 * G) + vc * (4 * G)), 4 * G);
-        __builtin_memcpy(vd, P.v + at + sc + (off + 4 * quad) * (2 * G), 8 * G);
+        if (W == 4) {
+            __builtin_memcpy(code[0], P.k + at + (uint32_t)((off + kt) * (16 * G) + kc * (4 * G)), 4 * G);
+            __builtin_memcpy(scale[0], P.k + at + sc + (off + kt) * (2 * G), 2 * G);
+            __builtin_memcpy(code[SETS - 1], P.v + at + (uint32_t)(off * (16 * G) + quad * (64 * G) + vc * (4 * G)),
+                             4 * G);
+            __builtin_memcpy(scale[SETS - 1], P.v + at + sc + (off + 4 * quad) * (2 * G), 8 * G);
+        } else {
+            const uint8_t *pool = wave < 4 ? P.k : P.v;
+            const uint32_t c = wave < 4 ? (uint32_t)(kt * (16 * G) + kc * (4 * G)) : (uint32_t)(quad * (64 * G) + vc * (4 * G));
+            const uint32_t d = wave < 4 ? (uint32_t)(kt * (2 * G)) : (uint32_t)(4 * quad * (2 * G));
+            __builtin_memcpy(code[0], pool + at + off * (16 * G) + c, 4 * G);
+            if (wave < 4)
+                __builtin_memcpy(scale[0], pool + at + sc + off * (2 * G) + d, 2 * G);
+            else
+                __builtin_memcpy(scale[0], pool + at + sc + off * (2 * G) + d, 8 * G);
+        }
     };
     if (s_lo < s_hi) {
         look(s_lo);
@@ -674,8 +697,10 @@ __global__ __launch_bounds__(256, G == 8 || F32 ? 1 : 2) void paged_attn_tile_ke
         big = fmaxf(big, __shfl_xor(big, 32, 64));
         int e = 0;
         if (big > 0.0f && big < __builtin_inff()) (void)frexpf(big, &e);
-        qf = A.scale * ldexpf(1.0f, e);
-        const float down = ldexpf(1.0f, -(e >> 1)), more = ldexpf(1.0f, -(e - (e >> 1)));
+        // qf > 0, so that a maximum of products is one of scores
+        qf = fmaxf(fabsf(A.scale) * ldexpf(1.0f, e), 1.17549435e-38f);
+        const float down = ldexpf(1.0f, -(e >> 1)), sign = A.scale > 0.0f ? 1.0f : A.scale < 0.0f ? -1.0f : 0.0f;
+        const float more = ldexpf(sign, -(e - (e >> 1)));
         const int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
 #pragma unroll
         for (int k = 0; k < 2 * G; k++)
@@ -689,7 +714,7 @@ __global__ __launch_bounds__(256, G == 8 || F32 ? 1 : 2) void paged_attn_tile_ke
 
     float m = -__builtin_inff(), l = 0.0f;
     int E = 0;
-    uint32_t limit = 0;  // the halves' bits of the largest |d| that E holds
+    uint32_t limit = 0;  // the half's bits of the largest |d| that E holds
     f32x16v acc[G];
 #pragma unroll
     for (int g = 0; g < G; g++)
@@ -698,82 +723,75 @@ __global__ __launch_bounds__(256, G == 8 || F32 ? 1 : 2) void paged_attn_tile_ke
     const int full_lo = rg.lo + (A.window > 0 ? n_tok - 1 : 0), full_hi = rg.hi - (n_tok - 1);
     const PagedMagic magic;
 
-    for (int s = s_lo; s < s_hi; s++) {
-        const int t0 = rg.first + s * 64;
-        // scales of tokens that no row sees become 0; the largest of the others
-        const bool all = t0 + 16 * wave >= rg.lo && t0 + 16 * wave + 16 <= rg.hi && here;
-        if (!all) {
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int t = t0 + 16 * wave + 4 * quad + r;
-                const bool out = t < rg.lo || t >= rg.hi || !here;
-#pragma unroll
-                for (int g = 0; g < G; g++) {
-                    const int e = r * G + g;
-                    vd[e >> 1] &= out ? (e & 1 ? 0x0000FFFFu : 0xFFFF0000u) : 0xFFFFFFFFu;
-                }
-            }
-        }
+    // Before the barrier in front of a step's unpacking: the values' scales that no
+    // row sees become 0, the largest of the others and the page's presence are told.
+    auto tell = [&](int s) __attribute__((always_inline)) {
+        uint32_t(&vd)[2 * G] = scale[SETS - 1];
         uint32_t most = 0;
+        const int t0 = rg.first + s * 64 + 16 * w4;
+        if (do_v) {
+            if (!(t0 >= rg.lo && t0 + 16 <= rg.hi && here)) {
 #pragma unroll
-        for (int j = 0; j < 2 * G; j++) {
-            const uint32_t a = vd[j] & 0x7FFFu, b = (vd[j] >> 16) & 0x7FFFu;
-            most = most > a ? most : a;
-            most = most > b ? most : b;
-        }
-        if (__ballot(most > limit)) {
-            for (int o = 32; o > 0; o >>= 1) {
-                const uint32_t y = (uint32_t)__shfl_xor((int)most, o, 64);
-                most = most > y ? most : y;
-            }
-        }
-        if (lane == 0) s_most[wave] = most;
-        __syncthreads();  // and every wave has read the step before
-        uint32_t top = s_most[0];
-#pragma unroll
-        for (int w = 1; w < 4; w++) top = top > s_most[w] ? top : s_most[w];
-        top = (uint32_t)uniform((int)top);
-        bool bad = false;
-        if (top > limit) {
-            bad = top >= 0x7C00u;  // NaN or infinity among them
-            if (bad) {
-                // those groups become 0 here and NaN to the rows that see them
-#pragma unroll
-                for (int r = 0; r < 4; r++)
+                for (int r = 0; r < 4; r++) {
+                    const int t = t0 + 4 * quad + r;
+                    const bool out = t < rg.lo || t >= rg.hi || !here;
 #pragma unroll
                     for (int g = 0; g < G; g++) {
                         const int e = r * G + g;
-                        const uint32_t w = (vd[e >> 1] >> (16 * (e & 1))) & 0x7FFFu;
-                        if (vc == 0) s_bad[16 * wave + 4 * quad + r][g] = w >= 0x7C00u;
-                        if (w >= 0x7C00u) vd[e >> 1] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                        vd[e >> 1] &= out ? (e & 1 ? 0x0000FFFFu : 0xFFFF0000u) : 0xFFFFFFFFu;
                     }
-                top = 0x7BFFu;
-            }
-            if (top > limit) {
-                // |d| < 2^e, d 2^E <= 2^12, |d (c - 8)| 2^E <= 2^15
-                int e;
-                (void)frexpf(h2f((uint16_t)top), &e);
-                const int was = E;
-                E = 12 - e;
-                limit = 0x7BFFu;
-                if (e < 15) limit = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)ldexpf(1.0f, e));
-                if (m != -__builtin_inff()) {
-                    const float a = ldexpf(1.0f, E - was);
-#pragma unroll
-                    for (int g = 0; g < G; g++) acc[g] *= a;
                 }
             }
+            typedef uint16_t u16x2v __attribute__((ext_vector_type(2)));
+            u16x2v top = {0, 0};
+#pragma unroll
+            for (int j = 0; j < 2 * G; j++) {
+                const uint32_t a = vd[j] & 0x7FFF7FFFu;
+                top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2v, a));
+            }
+            most = top[0] > top[1] ? top[0] : top[1];
+            if (__ballot(most > limit)) {
+                for (int o = 32; o > 0; o >>= 1) {
+                    const uint32_t y = (uint32_t)__shfl_xor((int)most, o, 64);
+                    most = most > y ? most : y;
+                }
+            }
+            if (lane == 0) s_most[s & 1][w4] = most;
         }
-        // unpack: keys of token kt, channels 32 g + 8 kc ..; values of quad `quad`,
-        // channels 32 g + vc and 32 g + 16 + vc
-        {
-            const int t = 16 * wave + kt;
+        if (do_k && lane == 0) s_page[s & 1][w4] = here;
+    };
+    // Behind it: E and the pages of the step.  True where some scales are NaN or
+    // infinite.
+    bool pages[4], pages_next[4] = {};
+    auto decide = [&](int s, int *e_new) __attribute__((always_inline)) {
+#pragma unroll
+        for (int w = 0; w < 4; w++) pages_next[w] = uniform((int)s_page[s & 1][w]) != 0;
+        uint32_t top = s_most[s & 1][0];
+#pragma unroll
+        for (int w = 1; w < 4; w++) top = top > s_most[s & 1][w] ? top : s_most[s & 1][w];
+        top = (uint32_t)uniform((int)top);
+        *e_new = E;
+        if (top <= limit) return false;
+        const bool bad = top >= 0x7C00u;
+        if (bad) top = 0x7BFFu;
+        if (top > limit) {
+            // |d| < 2^e, |d| 2^E <= 2^12, |d (c - 8)| 2^E <= 2^15
+            int e;
+            (void)frexpf(h2f((uint16_t)top), &e);
+            *e_new = 12 - e < 30 ? 12 - e : 30;
+            limit = e < 15 ? (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)ldexpf(1.0f, e)) : 0x7BFFu;
+        }
+        return bad;
+    };
+    auto unpack = [&](int s, int b, int e_new, bool bad) __attribute__((always_inline)) {
+        if (do_k) {  // token kt's channels 32 g + 8 kc ..
+            const int t = 16 * w4 + kt;
 #pragma unroll
             for (int g = 0; g < G; g++) {
-                const _Float16 d = paged_h2(kd[g >> 1])[g & 1];
+                const _Float16 d = paged_h2(scale[0][g >> 1])[g & 1];
                 const half2v d2 = {d, d};
                 // in the order 0 4 1 5 2 6 3 7 of each eight channels, as the queries
-                const u32x4v c = __builtin_bit_cast(u32x4v, magic.k8(kr[g]));
+                const u32x4v c = __builtin_bit_cast(u32x4v, magic.k8(code[0][g]));
                 u32x4v hi, lo;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
@@ -787,11 +805,32 @@ __global__ __launch_bounds__(256, G == 8 || F32 ? 1 : 2) void paged_attn_tile_ke
                         lo[j] = __builtin_bit_cast(uint32_t, r);
                     }
                 }
-                *(u32x4v *)&s_k[0][t][32 * g + 8 * kc] = hi;
-                if (F32) *(u32x4v *)&s_k[N - 1][t][32 * g + 8 * kc] = lo;
+                s_k[b][0][k_at(t, 4 * g + kc)] = __builtin_bit_cast(half8v, hi);
+                if (F32) s_k[b][N - 1][k_at(t, 4 * g + kc)] = __builtin_bit_cast(half8v, lo);
             }
-            const int at = 16 * wave + 4 * (2 * (quad & 1) + (quad >> 1));
-            const float up = ldexpf(1.0f, E);
+        }
+        if (do_v) {  // quad's four tokens, channels 32 g + vc and 32 g + 16 + vc
+            uint32_t(&vd)[2 * G] = scale[SETS - 1];
+            uint32_t(&vr)[G] = code[SETS - 1];
+            if (bad) {
+                // such groups become 0 here and NaN to the rows that see them
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int g = 0; g < G; g++) {
+                        const int e = r * G + g;
+                        const bool is = ((vd[e >> 1] >> (16 * (e & 1))) & 0x7FFFu) >= 0x7C00u;
+                        if (vc == 0) s_bad[s & 1][16 * w4 + 4 * quad + r][g] = is;
+                        vd[e >> 1] &= is ? (e & 1 ? 0x0000FFFFu : 0xFFFF0000u) : 0xFFFFFFFFu;
+                    }
+            }
+            // d 2^E in two exact steps (E - E / 2 <= 15)
+            const _Float16 u1 = (_Float16)ldexpf(1.0f, e_new / 2), u2 = (_Float16)ldexpf(1.0f, e_new - e_new / 2);
+            const half2v up1 = {u1, u1}, up2 = {u2, u2};
+            uint32_t dv[2 * G];
+#pragma unroll
+            for (int j = 0; j < 2 * G; j++) dv[j] = __builtin_bit_cast(uint32_t, paged_h2(vd[j]) * up1 * up2);
+            const int piece = 2 * w4 + (quad & 1);
 #pragma unroll
             for (int g = 0; g < G; g++) {
                 uint32_t hi[2][2], lo[2][2];
@@ -801,10 +840,9 @@ __global__ __launch_bounds__(256, G == 8 || F32 ? 1 : 2) void paged_attn_tile_ke
                     const uint32_t w = __builtin_amdgcn_perm(vr[b1 >> 2], vr[b0 >> 2],
                                                              0x0C000C00u | (uint32_t)(b0 & 3) |
                                                                  (uint32_t)(4 + (b1 & 3)) << 16);
-                    // d 2^E as a float (the half may be subnormal), exact as a half
-                    const float d0 = (float)paged_h2(vd[b0 >> 1])[b0 & 1] * up;
-                    const float d1 = (float)paged_h2(vd[b1 >> 1])[b1 & 1] * up;
-                    const half2v dd = {(_Float16)d0, (_Float16)d1};
+                    const half2v dd = paged_h2(__builtin_amdgcn_perm(dv[b1 >> 1], dv[b0 >> 1],
+                                                                     (b0 & 1 ? 0x0302u : 0x0100u) |
+                                                                         (b1 & 1 ? 0x07060000u : 0x05040000u)));
                     const uint32_t cw[2] = {magic.low(w), magic.high(w)};
 #pragma unroll
                     for (int n = 0; n < 2; n++) {
@@ -820,50 +858,78 @@ __global__ __launch_bounds__(256, G == 8 || F32 ? 1 : 2) void paged_attn_tile_ke
                 }
 #pragma unroll
                 for (int n = 0; n < 2; n++) {
-                    *(uint2 *)&s_v[0][32 * g + 16 * n + vc][at] = make_uint2(hi[n][0], hi[n][1]);
-                    if (F32) *(uint2 *)&s_v[N - 1][32 * g + 16 * n + vc][at] = make_uint2(lo[n][0], lo[n][1]);
+                    const int at = v_at(32 * g + 16 * n + vc, piece);
+                    ((uint2 *)&s_v[b][0][at])[quad >> 1] = make_uint2(hi[n][0], hi[n][1]);
+                    if (F32) ((uint2 *)&s_v[b][N - 1][at])[quad >> 1] = make_uint2(lo[n][0], lo[n][1]);
                 }
             }
         }
-        if (lane == 0) s_page[wave] = here;
-        if (((s + 1 - s_lo) & 63) == 0 && s + 1 < s_hi) look(s + 1);
-        load(s + 1 < s_hi ? s + 1 : s);
-        __syncthreads();
+    };
+    // the load behind a step's unpacking (the last step's is not used)
+    auto load_next = [&](int s) __attribute__((always_inline)) {
+        if (((s - s_lo) & 63) == 0 && s < s_hi) look(s);
+        load(s < s_hi ? s : s_hi - 1);
+    };
 
-        bool pages[4];
+    bool bad = false, bad_next = false;
+    int e_next = 0;
+    if (s_lo < s_hi) {
+        tell(s_lo);
+        __syncthreads();
+        bad = decide(s_lo, &E);
+        unpack(s_lo, s_lo & (NB - 1), E, bad);
+        load_next(s_lo + 1);
+    }
+    for (int s = s_lo; s < s_hi; s++) {
+        const int t0 = rg.first + s * 64, b = s & (NB - 1);
+        const bool more = s + 1 < s_hi;
+        if (more) tell(s + 1);
+        __syncthreads();  // step s is in LDS; nobody reads step s - 1 any more
 #pragma unroll
-        for (int w = 0; w < 4; w++) pages[w] = uniform((int)s_page[w]) != 0;
+        for (int w = 0; w < 4; w++) pages[w] = pages_next[w];
         const bool full = t0 >= full_lo && t0 + 64 <= full_hi && pages[0] && pages[1] && pages[2] && pages[3];
+        e_next = E;
+        if (more) bad_next = decide(s + 1, &e_next);
+
         // scores of 64 tokens: [32-token tile][16]
         f32x16v sc[2];
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
+        for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int i = 0; i < 16; i++) sc[u][i] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 2 * G; k++) {
-                const half8v a = *(const half8v *)&s_k[0][32 * u + col][16 * k + 8 * half];
+        for (int k = 0; k < 2 * G; k++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const half8v a = s_k[b][0][k_at(32 * u + col, 2 * k + half)];
                 sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[0][k], sc[u], 0, 0, 0);
                 if (F32) {
-                    const half8v b = *(const half8v *)&s_k[N - 1][32 * u + col][16 * k + 8 * half];
+                    const half8v c = s_k[b][N - 1][k_at(32 * u + col, 2 * k + half)];
                     sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[N - 1][k], sc[u], 0, 0, 0);
-                    sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, q[0][k], sc[u], 0, 0, 0);
+                    sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(c, q[0][k], sc[u], 0, 0, 0);
                 }
             }
+        if (NB == 2 && more) {
+            unpack(s + 1, b ^ 1, e_next, bad_next);
+            load_next(s + 2);
         }
-        float mx = -__builtin_inff();
+        if (!full) {
+            const float none = -__builtin_inff();
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int t = t0 + 32 * u + 8 * (i >> 2) + 4 * half + (i & 3);
+                    const bool in = (t >= rlo) & (t < rhi) & pages[2 * u + (i >> 3)];
+                    sc[u][i] = in ? sc[u][i] : none;
+                }
+        }
+        float mx = sc[0][0];
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                sc[u][i] *= qf;
-                if (!full) {
-                    const int k = 32 * u + 8 * (i >> 2) + 4 * half + (i & 3), t = t0 + k;
-                    const bool page = pages[2 * u + (i >> 3)];
-                    if (t < rlo || t >= rhi || !page) sc[u][i] = -__builtin_inff();
-                }
-                mx = fmaxf(mx, sc[u][i]);
-            }
+            for (int i = 0; i < 16; i++) mx = fmaxf(mx, sc[u][i]);
+        mx *= qf;
         // m follows the maximum only when it is 8 behind: p 2^6 stays at or below 2^14,
         // and keeps all its bits as a half down to 2^-28 of that
         if (__ballot(mx > m + 8.0f || (m == -__builtin_inff() && mx > m))) {
@@ -876,36 +942,52 @@ __global__ __launch_bounds__(256, G == 8 || F32 ? 1 : 2) void paged_attn_tile_ke
             for (int g = 0; g < G; g++) acc[g] *= a;
         }
         const float base = (m == -__builtin_inff() ? 0.0f : m) - 6.0f;
-        half8v ph[4], pl[F32 ? 4 : 1];
+        float l4[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int u = 0; u < 2; u++)
+        for (int c = 0; c < 4; c++) {
+            half8v ph, pl;
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float p = __builtin_amdgcn_exp2f(sc[u][i] - base);
-                l += p;
-                ph[2 * u + (i >> 3)][i & 7] = (_Float16)p;
-                if (F32) pl[F32 ? 2 * u + (i >> 3) : 0][i & 7] = (_Float16)(p - (float)(_Float16)p);
+            for (int i = 0; i < 8; i++) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(sc[c >> 1][8 * (c & 1) + i], qf, -base));
+                l4[i & 3] += p;
+                ph[i] = (_Float16)p;
+                if (F32) pl[i] = (_Float16)(p - (float)(_Float16)p);
             }
-#pragma unroll
-        for (int g = 0; g < G; g++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const half8v a = *(const half8v *)&s_v[0][32 * g + col][16 * c + 8 * half];
-                acc[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[c], acc[g], 0, 0, 0);
-                if (F32) {
-                    const half8v b = *(const half8v *)&s_v[N - 1][32 * g + col][16 * c + 8 * half];
-                    acc[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[F32 ? c : 0], acc[g], 0, 0, 0);
-                    acc[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, ph[c], acc[g], 0, 0, 0);
-                }
-            }
-        if (bad) {
 #pragma unroll
             for (int g = 0; g < G; g++) {
-                bool sees = false;
-                for (int k = 0; k < 64; k++) sees |= s_bad[k][g] && t0 + k >= rlo && t0 + k < rhi;
-                if (sees) acc[g] += __builtin_nanf("");
+                const half8v a = s_v[b][0][v_at(32 * g + col, 2 * c + half)];
+                acc[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph, acc[g], 0, 0, 0);
+                if (F32) {
+                    const half8v d = s_v[b][N - 1][v_at(32 * g + col, 2 * c + half)];
+                    acc[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl, acc[g], 0, 0, 0);
+                    acc[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(d, ph, acc[g], 0, 0, 0);
+                }
             }
         }
+        l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+        if (bad) {
+#pragma unroll 1
+            for (int g = 0; g < G; g++) {
+                bool sees = false;
+#pragma unroll 1
+                for (int k = 0; k < 64; k++) sees |= s_bad[s & 1][k][g] && t0 + k >= rlo && t0 + k < rhi;
+                const float add = sees ? __builtin_nanf("") : 0.0f;
+#pragma unroll
+                for (int h = 0; h < G; h++) acc[h] += h == g ? add : 0.0f;
+            }
+        }
+        if (NB == 1 && more) {
+            __syncthreads();
+            unpack(s + 1, 0, e_next, bad_next);
+            load_next(s + 2);
+        }
+        if (e_next != E) {
+            const float a = ldexpf(1.0f, e_next - E);
+#pragma unroll
+            for (int g = 0; g < G; g++) acc[g] *= a;
+            E = e_next;
+        }
+        bad = bad_next;
     }
 
     l += __shfl_xor(l, 32, 64);
@@ -952,30 +1034,26 @@ __global__ __launch_bounds__(256, G == 8 || F32 ? 1 : 2) void paged_attn_tile_ke
         }
 }
 
-// Joins a row's splits.  One workgroup per (token, query head): the splits'
-// weights first, then each of 256 / DV groups of threads sums every so-manieth
-// split, eight loads in flight, and the groups' sums are added in their order.
+// Joins the splits of the sessions that are row tiles.  One workgroup per (session,
+// row of it, query head): the splits' weights first, then each of 256 / DV groups of
+// threads sums every so-manieth split, eight loads in flight, and the groups' sums
+// are added in their order.
 template <int G, bool F32>
-__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedDev P, PagedAttn A) {
+__global__ __launch_bounds__(256) void paged_attn_join_rows_kernel(PagedDev P, PagedAttn A) {
     constexpr int DV = 32 * G, N = 256 / DV;
     __shared__ float s_f[256], s_o[N][DV], s_red[4];
-    const int64_t rows = (int64_t)P.n_tokens * A.n_heads, w = blockIdx.x;
-    const int token = (int)(w / A.n_heads), hd = (int)(w % A.n_heads);
+    const uint32_t r = blockIdx.x / (uint32_t)A.n_heads;
+    const int hd = (int)(blockIdx.x - r * (uint32_t)A.n_heads);
+    const int seq = (int)(r / (uint32_t)A.short_q), tk = (int)(r - (uint32_t)seq * (uint32_t)A.short_q);
+    const int a = P.q_starts[seq], b = P.q_starts[seq + 1];
+    if (a < 0 || b > P.n_tokens || tk >= b - a || (A.both && b - a > A.short_q)) return;
+    const int64_t rows = (int64_t)P.n_tokens * A.n_heads, token = a + tk, w = token * A.n_heads + hd;
     const int i = threadIdx.x;  // at most 256 splits
-    const int most = A.n_splits > A.tile_splits ? A.n_splits : A.tile_splits;
     float m = -__builtin_inff(), part = 0.0f;
-    if (i < most) {
+    if (i < A.n_splits) {
         m = A.ml[(i * rows + w) * 2];
         part = A.ml[(i * rows + w) * 2 + 1];
     }
-    int seq, a, b;
-    // rows of no tile stay as they are, rows of one split are done
-    if (!paged_session(P, token, &seq, &a, &b)) return;
-    const bool tiled = A.short_q == 0 || (A.both && b - a > A.short_q);
-    if (!tiled && token - a >= A.short_q) return;
-    const int n_splits = tiled ? A.tile_splits : A.n_splits;
-    if (n_splits <= 1) return;
-    if (i >= n_splits) m = -__builtin_inff();
     const float top = block_max_256(m, s_red);
     const bool none = top == -__builtin_inff();
     float base = none ? 0.0f : top, sink = 0.0f;
@@ -989,12 +1067,12 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedDev P, PagedA
     const float sum = block_sum_256(f == 0.0f ? 0.0f : f * part, s_red) + sink;  // the barriers order s_f too
     const int ch = i % DV;
     float o[4] = {0, 0, 0, 0};
-    for (int s = i / DV; s < n_splits; s += 8 * N) {
+    for (int s = i / DV; s < A.n_splits; s += 8 * N) {
         float x[8], f8[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const int at = s + j * N < n_splits ? s + j * N : 0;
-            f8[j] = s + j * N < n_splits ? s_f[at] : 0.0f;
+            const int at = s + j * N < A.n_splits ? s + j * N : 0;
+            f8[j] = s + j * N < A.n_splits ? s_f[at] : 0.0f;
             x[j] = A.part[(at * rows + w) * DV + ch];
         }
 #pragma unroll
@@ -1013,6 +1091,62 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedDev P, PagedA
         ((float *)A.out)[to] = y;
     else
         ((uint16_t *)A.out)[to] = f32_to_bf16(y);
+}
+
+// The same for the rows of larger tiles, of which there are many with few splits:
+// one wave per (row, query head).
+template <int G, bool F32>
+__global__ __launch_bounds__(256) void paged_attn_join_tiles_kernel(PagedDev P, PagedAttn A) {
+    constexpr int DV = 32 * G, N = DV / 64;
+    const int lane = threadIdx.x & 63;
+    const int64_t rows = (int64_t)P.n_tokens * A.n_heads, w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (w >= rows) return;
+    const int token = (int)(w / A.n_heads), hd = (int)(w - (int64_t)token * A.n_heads);
+    int seq, a, b;
+    // rows of no session stay as they are
+    if (!paged_session(P, token, &seq, &a, &b) || (A.both && b - a <= A.short_q)) return;
+    float top = -__builtin_inff();
+    for (int s = lane; s < A.n_splits; s += 64) top = fmaxf(top, A.ml[(s * rows + w) * 2]);
+    top = wave_max(top);
+    const bool none = top == -__builtin_inff();
+    float base = none ? 0.0f : top, sum = 0.0f;
+    if (A.sinks) {
+        const float sink = A.sinks[hd] * 1.44269504f;
+        base = none ? sink : fmaxf(base, sink);
+        sum = __builtin_amdgcn_exp2f(sink - base);
+    }
+    float o[N] = {};
+    for (int s = 0; s < A.n_splits; s += 4) {
+        float x[4][N], m[4], l[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int64_t at = (s + j < A.n_splits ? s + j : s) * rows + w;
+            m[j] = A.ml[at * 2];
+            l[j] = A.ml[at * 2 + 1];
+#pragma unroll
+            for (int n = 0; n < N; n++) x[j][n] = A.part[at * DV + lane + 64 * n];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            // a split without keys wrote no sums
+            const bool has = s + j < A.n_splits && m[j] != -__builtin_inff();
+            const float f = has ? __builtin_amdgcn_exp2f(m[j] - base) : 0.0f;
+            sum = has ? fmaf(f, l[j], sum) : sum;
+#pragma unroll
+            for (int n = 0; n < N; n++) o[n] = has ? fmaf(f, x[j][n], o[n]) : o[n];
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        const int ch = lane + 64 * n;
+        if (ch >= P.vd) continue;
+        const float y = none ? 0.0f : o[n] / sum;
+        const int64_t to = token * A.o_stride + (int64_t)hd * P.vd + ch;
+        if (F32)
+            ((float *)A.out)[to] = y;
+        else
+            ((uint16_t *)A.out)[to] = f32_to_bf16(y);
+    }
 }
 
 }  // namespace rh

@@ -4469,10 +4469,10 @@ struct PagedDevice {
 };
 
 // How a call's attention is cut.  Sessions of few rows (R of tokens x query heads of
-// a kv head) are a row tile each; the others are tiles of 128 rows.
+// a kv head) are a row tile each; the others are tiles of 32 rows per wave.
 struct PagedPlan {
     int R = 0, W = 0, short_q = 0, splits = 1, steps = 0;  // row tiles, short_q = 0: none
-    int tok_tile = 0, tile_splits = 1, tile_steps = 0;     // 128-row tiles, tok_tile = 0: none
+    int waves = 0, tok_tile = 0, tile_splits = 1, tile_steps = 0;  // larger tiles, tok_tile = 0: none
     int64_t tiles = 0, heads_y = 0;
 };
 static PagedPlan paged_plan(const PagedDev &P, uint32_t n_heads, uint32_t max_q, uint32_t max_kv, uint32_t window) {
@@ -4509,11 +4509,15 @@ static PagedPlan paged_plan(const PagedDev &P, uint32_t n_heads, uint32_t max_q,
         p.steps = (int)per;
     }
     if (tiles) {
-        p.tok_tile = 128 / chunk;
+        // 8 waves share the unpacking of keys and values twice as far as 4; sessions of
+        // up to 128 rows would leave half of them idle, and two steps of 256 channels
+        // fill the registers of 4
+        p.waves = P.hd > 128 || P.vd > 128 || (int64_t)max_q * chunk <= 128 ? 4 : 8;
+        p.tok_tile = 32 * p.waves / chunk;
         p.tiles = P.n_tokens / p.tok_tile + (int64_t)P.n_seqs;
-        // two workgroups per CU, of 4 steps or more each
+        // eight waves per CU, of 4 steps or more each
         const int64_t steps = steps_of(p.tok_tile), items = (P.n_tokens + p.tok_tile - 1) / p.tok_tile * p.heads_y;
-        int64_t n = 512 / items;
+        int64_t n = 256 * 8 / p.waves / items;
         if (n > (steps + 3) / 4) n = (steps + 3) / 4;
         if (n < 1) n = 1;
         if (n > 256) n = 256;
@@ -4554,7 +4558,13 @@ static void paged_attn_launch(const PagedDev &P, PagedAttn A, const PagedPlan &p
     if (p.tok_tile) {
         tiles_of(p.tok_tile, p.tile_splits, p.tile_steps, 1 << 16);
         const dim3 grid((unsigned)(p.tiles * p.heads_y), (unsigned)p.tile_splits);
-        paged_attn_tile_kernel<G, F32><<<grid, 256, 0, s>>>(P, A);
+        if (p.waves == 4)
+            paged_attn_tile_kernel<G, F32, 4><<<grid, 256, 0, s>>>(P, A);
+        else if constexpr (G != 8)
+            paged_attn_tile_kernel<G, F32, 8><<<grid, 512, 0, s>>>(P, A);
+        if (p.tile_splits > 1)
+            paged_attn_join_tiles_kernel<G, F32>
+                <<<(unsigned)(((int64_t)P.n_tokens * A.n_heads + 3) / 4), 256, 0, s>>>(P, A);
     }
     if (p.short_q) {
         tiles_of(p.short_q, p.splits, p.steps, 1 << 8);
@@ -4562,10 +4572,8 @@ static void paged_attn_launch(const PagedDev &P, PagedAttn A, const PagedPlan &p
             paged_attn_rows_launch<G, F32, 1>(P, A, p, s);
         else
             paged_attn_rows_launch<G, F32, 4>(P, A, p, s);
-    }
-    if (p.splits > 1 || p.tile_splits > 1) {
-        A.n_splits = p.splits;
-        paged_attn_join_kernel<G, F32><<<(unsigned)((int64_t)P.n_tokens * A.n_heads), 256, 0, s>>>(P, A);
+        if (p.splits > 1)
+            paged_attn_join_rows_kernel<G, F32><<<(unsigned)(P.n_seqs * p.short_q * A.n_heads), 256, 0, s>>>(P, A);
     }
 }
 
@@ -4706,7 +4714,8 @@ int rusty_hip_paged_attention(const RustyPagedKv *kv, const RustyPagedBatch *bat
     const PagedPlan p = paged_plan(P, rows->n_heads, batch->max_q_len, batch->max_kv_len, rows->window);
     const uint64_t need = paged_workspace(P, p, rows->n_heads);
     if (need && (!rows->workspace || rows->workspace_len < need || (uintptr_t)rows->workspace % 16)) return 0;
-    if (p.tiles * p.heads_y > (0x7FFFFFFF >> 8) || P.n_seqs * p.heads_y > (0x7FFFFFFF >> 8) || (int64_t)n * rows->n_heads > 0x7FFFFFFF) return 0;
+    if (p.tiles * p.heads_y > (0x7FFFFFFF >> 8) || P.n_seqs * p.heads_y > (0x7FFFFFFF >> 8) ||
+        (int64_t)P.n_seqs * p.short_q * rows->n_heads > (0x7FFFFFFF >> 8) || (int64_t)n * rows->n_heads > 0x7FFFFFFF) return 0;
     PagedAttn A;
     A.q = rows->q;
     A.out = rows->out;
@@ -4723,7 +4732,6 @@ int rusty_hip_paged_attention(const RustyPagedKv *kv, const RustyPagedBatch *bat
     A.window = (int)rows->window;
     A.short_q = p.short_q;
     A.both = p.short_q && p.tok_tile;
-    A.tile_splits = p.tile_splits;
     hipStream_t s = (hipStream_t)stream;
     const int G = paged_groups(P.hd, P.vd);
     if (rows->dtype)
