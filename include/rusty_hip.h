@@ -353,17 +353,17 @@ typedef struct {
     const int32_t *q_starts;    /* [n_seqs + 1] */
     uintptr_t page_table_len, kv_lens_len, q_starts_len; /* bytes */
     uint32_t n_seqs, table_stride;
-    uint32_t n_rows;            /* rows of the call's row buffers, the last session's end or more */
     uint32_t max_q_len;         /* most rows of a session: later rows of one are not attended for */
     uint32_t max_kv_len;        /* about the longest session; sizes the work's split, any value is correct */
 } RustyPagedBatch;
 
-/* Row buffers: row r of x starts at x + r * x_stride elements (float, or bf16
+/* Row buffers: n_rows rows each, the last session's end or more; row r of x starts at x + r * x_stride elements (float, or bf16
  * with dtype = 1); rows are [heads][dim] without gaps.  Bases are aligned to
  * four elements, strides are multiples of four.  x_len: bytes from x that the
  * call may touch. */
 typedef struct {
     uint32_t dtype;             /* of all rows: 0 = f32, 1 = bf16 */
+    uint32_t n_rows;
     uint32_t n_heads;           /* query heads (0 without q) */
     const void *q, *k, *v;      /* q may be null: keys and values only */
     void *q_out;                /* rotated queries, may be q itself */
@@ -378,6 +378,7 @@ typedef struct {
 
 typedef struct {
     uint32_t dtype;
+    uint32_t n_rows;
     void *k, *v;                /* [n_kv_heads][head_dim] / [value_dim] rows; one may be null */
     uintptr_t k_len, v_len;
     int64_t k_stride, v_stride;
@@ -385,6 +386,7 @@ typedef struct {
 
 typedef struct {
     uint32_t dtype;
+    uint32_t n_rows;
     uint32_t n_heads;           /* a multiple of n_kv_heads */
     const void *q;
     void *out;                  /* [n_heads][value_dim] rows */
@@ -414,7 +416,8 @@ int rusty_hip_paged_read(const RustyPagedKv *kv, const RustyPagedBatch *batch, c
                          void *stream);
 /* Workspace bytes of rusty_hip_paged_attention for this batch's sizes (the
  * pointers are not looked at); 0 if none is needed or the sizes are not taken. */
-uint64_t rusty_hip_paged_attention_workspace(const RustyPagedKv *kv, const RustyPagedBatch *batch, uint32_t n_heads);
+uint64_t rusty_hip_paged_attention_workspace(const RustyPagedKv *kv, const RustyPagedBatch *batch, uint32_t n_rows,
+                                             uint32_t n_heads);
 /* Softmax attention of the rows' queries over their session's cached positions,
  * causal from each row's own position, with sliding window and per-head sinks
  * (as rusty_hip_attention).  A row whose masks leave nothing is 0.  Sums,

@@ -69,23 +69,40 @@ __device__ __forceinline__ bool paged_session(const PagedDev &P, int t, int *seq
     return t >= *start && t < *end;
 }
 
-// Session and position of row t: a session's rows are its last ones.  False also
-// for negative positions.
-__device__ __forceinline__ bool paged_row(const PagedDev &P, int t, int *seq, int *pos) {
-    int a, b;
-    if (!paged_session(P, t, seq, &a, &b)) return false;
-    const int64_t p = (int64_t)P.kv_lens[*seq] - ((int64_t)b - t);
-    *pos = (int)p;
-    return p >= 0;
+// Session and position of the N rows from t on (a session's rows are its last
+// ones), -1 for rows of no session and for positions below zero.  One pass over the
+// starts, and the N rows' loads in flight together.
+template <int N>
+__device__ __forceinline__ void paged_rows(const PagedDev &P, int t, int *seq, int *pos) {
+    const int lane = threadIdx.x & 63;
+    int n[N] = {};
+    for (int base = 0; base <= P.n_seqs; base += 64) {
+        const int i = base + lane, start = P.q_starts[i <= P.n_seqs ? i : 0];
+#pragma unroll
+        for (int j = 0; j < N; j++) n[j] += __popcll(__ballot(i <= P.n_seqs && start <= t + j));
+    }
+    int a[N], b[N], len[N];
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        seq[j] = n[j] > 0 && n[j] <= P.n_seqs ? n[j] - 1 : 0;
+        a[j] = P.q_starts[seq[j]];
+        b[j] = P.q_starts[seq[j] + 1];
+        len[j] = P.kv_lens[seq[j]];
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        const int64_t p = (int64_t)len[j] - ((int64_t)b[j] - (t + j));
+        const bool ok = n[j] > 0 && n[j] <= P.n_seqs && t + j < P.n_tokens && t + j >= a[j] && t + j < b[j] && p >= 0;
+        pos[j] = ok ? (int)p : -1;
+    }
 }
 
 // Page of a position, or -1: outside the table's row or the pool.  *off: token in it.
 __device__ __forceinline__ int paged_page(const PagedDev &P, int seq, int pos, int *off) {
     const int i = page_of_tile(P, pos >> 4);
     *off = pos - i * P.ps;
-    if (i >= P.stride) return -1;
-    const int page = P.table[(int64_t)seq * P.stride + i];
-    return page >= 0 && page < P.n_pages ? page : -1;
+    const int page = P.table[(int64_t)seq * P.stride + (i < P.stride ? i : 0)];
+    return i < P.stride && page >= 0 && page < P.n_pages ? page : -1;
 }
 // wave-uniform values into scalar registers
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -191,8 +208,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedDev P, PagedAppe
     const int64_t w = (int64_t)blockIdx.x * 4 + wave;
     const int t = (int)(w / segs);
     int seg = (int)(w % segs);
+    if (t >= P.n_tokens) return;
     int seq, pos;
-    if (t >= P.n_tokens || !paged_row(P, t, &seq, &pos) || pos >= A.max_pos) return;
+    paged_rows<1>(P, t, &seq, &pos);
+    if (pos < 0 || pos >= A.max_pos) return;
     if (seg < A.q_segs) {
         // whole heads per wave: q_out may be q, where a lane's partner chunk is
         // another lane's output, and the wave's loads are all done before it stores
@@ -208,12 +227,12 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedDev P, PagedAppe
         return;
     }
     seg -= A.q_segs;
-    const bool is_v = seg >= A.kv_segs;
-    const int u = (is_v ? seg - A.kv_segs : seg) * 64 + lane;
-    const int head = u / (4 * G), g = (u % (4 * G)) >> 2, i = u & 3;
     int off;
     const int page = paged_page(P, seq, pos, &off);
     if (page < 0) return;
+    const bool is_v = seg >= A.kv_segs;
+    const int u = (is_v ? seg - A.kv_segs : seg) * 64 + lane;
+    const int head = u / (4 * G), g = (u % (4 * G)) >> 2, i = u & 3;
     const bool on = head < P.n_kv;
     uint8_t *blk = (is_v ? P.v : P.k) + ((int64_t)page * P.n_kv + (on ? head : 0)) * P.block;
     float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -264,58 +283,80 @@ struct PagedRead {
     int32_t kv_segs;
 };
 
-template <int G, class T>
+// One wave per (N rows, up to 64 dwords of keys or of values of each), the rows'
+// loads in flight together.  A lane puts out 16 bytes at a time, so that a store
+// covers 1 KB without gaps (eight f32 channels per lane, in two stores of every other
+// 16 bytes, took 53 us for 20001 rows instead of 50).
+template <int G, class T, int N>
 __global__ __launch_bounds__(256) void paged_read_kernel(PagedDev P, PagedRead A) {
-    __shared__ uint32_t s_v[4][64];
+    __shared__ uint32_t s_v[4][N][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t w = (int64_t)blockIdx.x * 4 + wave;
-    const int t = (int)(w / (2 * A.kv_segs));
-    const int seg = (int)(w % (2 * A.kv_segs));
-    int seq, pos;
-    if (t >= P.n_tokens || !paged_row(P, t, &seq, &pos)) return;
-    int off;
-    const int page = paged_page(P, seq, pos, &off);
-    if (page < 0) return;
+    const int t = (int)(w / (2 * A.kv_segs)) * N, seg = (int)(w % (2 * A.kv_segs));
+    if (t >= P.n_tokens) return;
     const bool is_v = seg >= A.kv_segs;
-    const int u = (is_v ? seg - A.kv_segs : seg) * 64 + lane;
-    const int head = u / (4 * G), g = (u % (4 * G)) >> 2, i = u & 3;
-    const bool on = head < P.n_kv;
-    const uint8_t *blk = (is_v ? P.v : P.k) + ((int64_t)page * P.n_kv + (on ? head : 0)) * P.block;
-    const float d = h2f(*(const uint16_t *)(blk + (int64_t)P.ps * (16 * G) + (off * G + g) * 2));
-    float x[8];
-    if (!is_v) {
-        const uint32_t word = *(const uint32_t *)(blk + (int64_t)off * (16 * G) + (i * G + g) * 4);
+    if (is_v ? !A.v : !A.k) return;
+    int seq[N], pos[N], page[N], off[N];
+    paged_rows<N>(P, t, seq, pos);
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = d * (float)((int)((word >> (4 * j)) & 15) - 8);
-        const int ch = 32 * g + 8 * i;
-        if (!on || !A.k || ch >= P.hd) return;
-        T *o = (T *)A.k + (int64_t)t * A.k_stride + (int64_t)head * P.hd + ch;
-        row_store4(o, x);
-        row_store4(o + 4, x + 4);
-        return;
+    for (int j = 0; j < N; j++) {  // (a row that has no page reads page 0)
+        page[j] = paged_page(P, seq[j], pos[j] < 0 ? 0 : pos[j], &off[j]);
+        if (pos[j] < 0) page[j] = -1;
+        if (page[j] < 0) off[j] = 0;
     }
-    const int b = (lane % (4 * G)) * 4, cc = b / G;
-    const uint8_t *src = blk + (int64_t)((off >> 2) * 64 + cc * 4 + (off & 3)) * G + b % G;
-    uint32_t word;
-    if (G >= 4)
-        word = *(const uint32_t *)src;
-    else
-        word = *(const uint16_t *)src | (uint32_t)*(const uint16_t *)(src + 4 * G) << 16;
-    s_v[wave][lane] = word;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    const uint8_t *s = (const uint8_t *)s_v[wave];
+    const uint8_t *pool = is_v ? P.v : P.k;
+    const int first = (is_v ? seg - A.kv_segs : seg) * (64 / (4 * G)), dim = is_v ? P.vd : P.hd;  // first head
+    const int64_t stride = is_v ? A.v_stride : A.k_stride;
+    T *out = (T *)(is_v ? A.v : A.k);
+    if (is_v) {
+        // [c][g] bytes of four channels' pairs to LDS
+        const int head = first + lane / (4 * G), b = (lane % (4 * G)) * 4, cc = b / G;
+        uint32_t word[N];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int q = s[(lane / (4 * G)) * (16 * G) + (4 * i + j) * G + g];
-        x[j] = d * (float)((q & 15) - 8);
-        x[4 + j] = d * (float)((q >> 4) - 8);
+        for (int j = 0; j < N; j++) {
+            const uint8_t *src = pool + ((int64_t)(page[j] < 0 ? 0 : page[j]) * P.n_kv + (head < P.n_kv ? head : 0)) * P.block +
+                                 (int64_t)((off[j] >> 2) * 64 + cc * 4 + (off[j] & 3)) * G + b % G;
+            if (G >= 4)
+                word[j] = *(const uint32_t *)src;
+            else
+                word[j] = *(const uint16_t *)src | (uint32_t)*(const uint16_t *)(src + 4 * G) << 16;
+        }
+#pragma unroll
+        for (int j = 0; j < N; j++) s_v[wave][j][lane] = word[j];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
-    const int ch = 32 * g + 4 * i;
-    if (!on || !A.v) return;
-    T *o = (T *)A.v + (int64_t)t * A.v_stride + (int64_t)head * P.vd + ch;
-    if (ch < P.vd) row_store4(o, x);
-    if (ch + 16 < P.vd) row_store4(o + 16, x + 4);
+    // C channels, 16 bytes of output, per lane and pass
+    constexpr int C = 16 / sizeof(T);
+#pragma unroll
+    for (int pass = 0; pass < 8 / C; pass++) {
+        const int u = 64 * pass + lane, head = first + u / (32 * G / C), r = u % (32 * G / C), g = r / (32 / C);
+        const int ch = r % (32 / C) * C;  // in the group
+        const bool on = head < P.n_kv && C * r < dim;
+        uint32_t code[N];
+        float d[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const uint8_t *blk = pool + ((int64_t)(page[j] < 0 ? 0 : page[j]) * P.n_kv + (head < P.n_kv ? head : 0)) * P.block;
+            d[j] = h2f(*(const uint16_t *)(blk + (int64_t)P.ps * (16 * G) + (off[j] * G + g) * 2));
+            const uint8_t *src = blk + (int64_t)off[j] * (16 * G) + ((ch >> 3) * G + g) * 4;
+            if (!is_v) code[j] = C == 8 ? *(const uint32_t *)src : *(const uint16_t *)(src + (ch & 4) / 2);
+        }
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            float x[C];
+            const uint8_t *s = (const uint8_t *)s_v[wave][j] + (u / (32 * G / C) * 16 + (ch & 15)) * G + g;
+#pragma unroll
+            for (int n = 0; n < C; n++) {
+                const uint32_t c = is_v ? (uint32_t)s[n * G] >> (ch >> 4) * 4 : code[j] >> (4 * n);
+                x[n] = d[j] * (float)((int)(c & 15) - 8);
+            }
+            if (!on || page[j] < 0) continue;
+            T *o = out + (int64_t)(t + j) * stride + (int64_t)head * dim + C * r;
+#pragma unroll
+            for (int n = 0; n < C; n += 4) row_store4(o + n, x + n);
+        }
+    }
 }
 
 }  // namespace rh

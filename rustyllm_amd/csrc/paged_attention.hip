@@ -758,14 +758,14 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void paged_attn_tile_kernel
             }
             if (lane == 0) s_most[s & 1][w4] = most;
         }
-        if (do_k && lane == 0) s_page[s & 1][w4] = here;
+        if (do_k && lane == 0) s_page[s & 1][w4] = here ? 1u << w4 : 0u;
     };
     // Behind it: E and the pages of the step.  True where some scales are NaN or
     // infinite.
-    bool pages[4], pages_next[4] = {};
+    uint32_t pages = 0, pages_next = 0;  // a bit per 16-token tile
     auto decide = [&](int s, int *e_new) __attribute__((always_inline)) {
-#pragma unroll
-        for (int w = 0; w < 4; w++) pages_next[w] = uniform((int)s_page[s & 1][w]) != 0;
+        const uint32_t *pg = s_page[s & 1];
+        pages_next = (uint32_t)uniform((int)(pg[0] | pg[1] | pg[2] | pg[3]));
         uint32_t top = s_most[s & 1][0];
 #pragma unroll
         for (int w = 1; w < 4; w++) top = top > s_most[s & 1][w] ? top : s_most[s & 1][w];
@@ -885,9 +885,8 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void paged_attn_tile_kernel
         const bool more = s + 1 < s_hi;
         if (more) tell(s + 1);
         __syncthreads();  // step s is in LDS; nobody reads step s - 1 any more
-#pragma unroll
-        for (int w = 0; w < 4; w++) pages[w] = pages_next[w];
-        const bool full = t0 >= full_lo && t0 + 64 <= full_hi && pages[0] && pages[1] && pages[2] && pages[3];
+        pages = pages_next;
+        const bool full = t0 >= full_lo && t0 + 64 <= full_hi && pages == 15;
         e_next = E;
         if (more) bad_next = decide(s + 1, &e_next);
 
@@ -920,7 +919,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void paged_attn_tile_kernel
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int t = t0 + 32 * u + 8 * (i >> 2) + 4 * half + (i & 3);
-                    const bool in = (t >= rlo) & (t < rhi) & pages[2 * u + (i >> 3)];
+                    const bool in = (t >= rlo) & (t < rhi) & ((pages >> (2 * u + (i >> 3))) & 1);
                     sc[u][i] = in ? sc[u][i] : none;
                 }
         }

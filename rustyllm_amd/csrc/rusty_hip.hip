@@ -166,7 +166,7 @@ static int init_locked() {
         sp = nullptr;
     }
     g.noalloc[g.dev] = (float *)sp;
-    g.state = 1;
+    __atomic_store_n(&g.state, 1, __ATOMIC_RELEASE);
     return 1;
 }
 
@@ -4408,12 +4408,12 @@ static uint64_t paged_bytes(uint32_t n_pages, uint32_t ps, uint32_t n_kv, uint32
 }
 
 // The sizes of a call's cache and batch, and their buffers unless sizes_only.
-static bool paged_dev(const RustyPagedKv *kv, const RustyPagedBatch *b, PagedDev *P, bool sizes_only) {
+static bool paged_dev(const RustyPagedKv *kv, const RustyPagedBatch *b, uint32_t n_rows, PagedDev *P, bool sizes_only) {
     if (!kv || !b) return false;
     const uint64_t need = paged_bytes(kv->n_pages, kv->page_size, kv->n_kv_heads, kv->head_dim, kv->value_dim);
     const uint32_t most = 1u << 24;  // rows, sessions and pages of a session
     if (!need || b->n_seqs == 0 || b->n_seqs > most || b->table_stride == 0 || b->table_stride > most ||
-        b->n_rows == 0 || b->n_rows > most || b->max_q_len == 0)
+        n_rows == 0 || n_rows > most || b->max_q_len == 0)
         return false;
     if (!sizes_only &&
         (!kv->k_pages || !kv->v_pages || kv->k_len < need || kv->v_len < need || (uintptr_t)kv->k_pages % 16 ||
@@ -4434,7 +4434,7 @@ static bool paged_dev(const RustyPagedKv *kv, const RustyPagedBatch *b, PagedDev
     P->vd = (int)kv->value_dim;
     P->n_seqs = (int)b->n_seqs;
     P->stride = (int)b->table_stride;
-    P->n_tokens = (int)b->n_rows;
+    P->n_tokens = (int)n_rows;
     P->block = (int64_t)kv->page_size * 18 * paged_groups(kv->head_dim, kv->value_dim);
     const uint32_t tiles = kv->page_size / 16;
     uint32_t log = 0;
@@ -4447,26 +4447,33 @@ static bool paged_dev(const RustyPagedKv *kv, const RustyPagedBatch *b, PagedDev
 // Launches run on the library's device, whichever is current in the caller's
 // thread; a stream of another device is refused.
 struct PagedDevice {
-    int before = -1;
+    int before = -1;  // the caller's device where another one had to be made current
     bool ok = false;
     explicit PagedDevice(hipStream_t s) {
-        {
+        if (__atomic_load_n(&g.state, __ATOMIC_ACQUIRE) != 1) {
+            int was = -1;
             std::lock_guard<std::mutex> lk(g.mu);
-            if (hipGetDevice(&before) != hipSuccess) before = -1;
-            ok = init_locked();
+            if (hipGetDevice(&was) != hipSuccess) was = -1;
+            if (!init_locked()) return;
+            if (was >= 0 && was != g.dev) before = was;  // the initialisation made g.dev current
         }
         int now = -1;
-        if (ok && (hipGetDevice(&now) != hipSuccess || now != g.dev)) ok = hipSetDevice(g.dev) == hipSuccess;
-        if (ok && s) {
-            hipDevice_t d = 0;
-            ok = hipStreamGetDevice(s, &d) == hipSuccess && (int)d == g.dev;
+        if (hipGetDevice(&now) != hipSuccess) return;
+        if (now != g.dev) {
+            if (hipSetDevice(g.dev) != hipSuccess) return;
+            before = now;
         }
+        hipDevice_t d = 0;
+        ok = !s || (hipStreamGetDevice(s, &d) == hipSuccess && (int)d == g.dev);
     }
     ~PagedDevice() {
-        int now = -1;
-        if (before >= 0 && (hipGetDevice(&now) != hipSuccess || now != before)) (void)hipSetDevice(before);
+        if (before >= 0) (void)hipSetDevice(before);
     }
 };
+
+// Four rows per wave of read where that still leaves four waves per SIMD (20001 rows:
+// 62 us with one, 53 with four; append, whose rows are larger, loses by it: 112, 122).
+static bool paged_quads(uint32_t n_rows) { return n_rows >= 2048; }
 
 // How a call's attention is cut.  Sessions of few rows (R of tokens x query heads of
 // a kv head) are a row tile each; the others are tiles of 32 rows per wave.
@@ -4509,10 +4516,12 @@ static PagedPlan paged_plan(const PagedDev &P, uint32_t n_heads, uint32_t max_q,
         p.steps = (int)per;
     }
     if (tiles) {
-        // 8 waves share the unpacking of keys and values twice as far as 4; sessions of
-        // up to 128 rows would leave half of them idle, and two steps of 256 channels
-        // fill the registers of 4
-        p.waves = P.hd > 128 || P.vd > 128 || (int64_t)max_q * chunk <= 128 ? 4 : 8;
+        // Two workgroups of 4 waves per CU overlap each other's products and
+        // exponentials; one of 8 unpacks keys and values half as often.  64-channel
+        // heads gain by the latter (a chunk of 400 tokens, 64 heads: 97 us a step,
+        // 100), 128-channel ones by the former (512 tokens: 33 us, 41); wider ones
+        // fill the registers of 4.
+        p.waves = P.hd > 64 || P.vd > 64 || (int64_t)max_q * chunk <= 128 ? 4 : 8;
         p.tok_tile = 32 * p.waves / chunk;
         p.tiles = P.n_tokens / p.tok_tile + (int64_t)P.n_seqs;
         // eight waves per CU, of 4 steps or more each
@@ -4590,9 +4599,9 @@ int rusty_hip_paged_append(const RustyPagedKv *kv, const RustyPagedBatch *batch,
                            void *stream) {
     using namespace rh;
     PagedDev P;
-    if (!rows || !paged_dev(kv, batch, &P, false) || rows->dtype > 1) return 0;
+    if (!rows || !paged_dev(kv, batch, rows->n_rows, &P, false) || rows->dtype > 1) return 0;
     const int item = rows->dtype ? 2 : 4;
-    const uint32_t n = batch->n_rows;
+    const uint32_t n = rows->n_rows;
     const int64_t kw = (int64_t)P.n_kv * P.hd, vw = (int64_t)P.n_kv * P.vd;
     if (!rows_ok(rows->k, rows->k_len, n, rows->k_stride, kw, item) ||
         !rows_ok(rows->v, rows->v_len, n, rows->v_stride, vw, item))
@@ -4654,9 +4663,9 @@ int rusty_hip_paged_read(const RustyPagedKv *kv, const RustyPagedBatch *batch, c
                          void *stream) {
     using namespace rh;
     PagedDev P;
-    if (!rows || !paged_dev(kv, batch, &P, false) || rows->dtype > 1 || (!rows->k && !rows->v)) return 0;
+    if (!rows || !paged_dev(kv, batch, rows->n_rows, &P, false) || rows->dtype > 1 || (!rows->k && !rows->v)) return 0;
     const int item = rows->dtype ? 2 : 4;
-    const uint32_t n = batch->n_rows;
+    const uint32_t n = rows->n_rows;
     if ((rows->k && !rows_ok(rows->k, rows->k_len, n, rows->k_stride, (int64_t)P.n_kv * P.hd, item)) ||
         (rows->v && !rows_ok(rows->v, rows->v_len, n, rows->v_stride, (int64_t)P.n_kv * P.vd, item)))
         return 0;
@@ -4669,15 +4678,18 @@ int rusty_hip_paged_read(const RustyPagedKv *kv, const RustyPagedBatch *batch, c
     A.k_stride = rows->k_stride;
     A.v_stride = rows->v_stride;
     A.kv_segs = (P.n_kv * 4 * G + 63) / 64;
-    const int64_t waves = (int64_t)n * 2 * A.kv_segs;
+    const bool quads = paged_quads(n);
+    const int64_t waves = (int64_t)(quads ? (n + 3) / 4 : n) * 2 * A.kv_segs;
     if ((waves + 3) / 4 > 0x7FFFFFFF) return 0;
     const unsigned grid = (unsigned)((waves + 3) / 4);
     hipStream_t s = (hipStream_t)stream;
-#define RH_PAGED_READ(GG)                                                 \
-    if (rows->dtype)                                                      \
-        paged_read_kernel<GG, uint16_t><<<grid, 256, 0, s>>>(P, A);       \
-    else                                                                  \
-        paged_read_kernel<GG, float><<<grid, 256, 0, s>>>(P, A)
+#define RH_PAGED_READ(GG)                                                                         \
+    if (rows->dtype)                                                                              \
+        quads ? paged_read_kernel<GG, uint16_t, 4><<<grid, 256, 0, s>>>(P, A)                     \
+              : paged_read_kernel<GG, uint16_t, 1><<<grid, 256, 0, s>>>(P, A);                    \
+    else                                                                                          \
+        quads ? paged_read_kernel<GG, float, 4><<<grid, 256, 0, s>>>(P, A)                        \
+              : paged_read_kernel<GG, float, 1><<<grid, 256, 0, s>>>(P, A)
     if (G == 2) {
         RH_PAGED_READ(2);
     } else if (G == 4) {
@@ -4690,10 +4702,11 @@ int rusty_hip_paged_read(const RustyPagedKv *kv, const RustyPagedBatch *batch, c
     return 1;
 }
 
-uint64_t rusty_hip_paged_attention_workspace(const RustyPagedKv *kv, const RustyPagedBatch *batch, uint32_t n_heads) {
+uint64_t rusty_hip_paged_attention_workspace(const RustyPagedKv *kv, const RustyPagedBatch *batch, uint32_t n_rows,
+                                             uint32_t n_heads) {
     using namespace rh;
     PagedDev P;
-    if (!paged_dev(kv, batch, &P, true) || !paged_heads_ok(P, n_heads)) return 0;
+    if (!paged_dev(kv, batch, n_rows, &P, true) || !paged_heads_ok(P, n_heads)) return 0;
     return paged_workspace(P, paged_plan(P, n_heads, batch->max_q_len, batch->max_kv_len, 0), n_heads);
 }
 
@@ -4701,9 +4714,9 @@ int rusty_hip_paged_attention(const RustyPagedKv *kv, const RustyPagedBatch *bat
                               void *stream) {
     using namespace rh;
     PagedDev P;
-    if (!rows || !paged_dev(kv, batch, &P, false) || rows->dtype > 1 || !paged_heads_ok(P, rows->n_heads)) return 0;
+    if (!rows || !paged_dev(kv, batch, rows->n_rows, &P, false) || rows->dtype > 1 || !paged_heads_ok(P, rows->n_heads)) return 0;
     const int item = rows->dtype ? 2 : 4;
-    const uint32_t n = batch->n_rows;
+    const uint32_t n = rows->n_rows;
     if (!rows_ok(rows->q, rows->q_len, n, rows->q_stride, (int64_t)rows->n_heads * P.hd, item) ||
         !rows_ok(rows->out, rows->out_len, n, rows->out_stride, (int64_t)rows->n_heads * P.vd, item) ||
         (rows->sinks && ((uintptr_t)rows->sinks % 4 || rows->sinks_len < (uint64_t)rows->n_heads * 4)) ||

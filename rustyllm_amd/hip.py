@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct as _struct
 
 import numpy as np
 
@@ -675,12 +676,12 @@ class _PagedKv(C.Structure):
 class _PagedBatch(C.Structure):
     _fields_ = [("page_table", C.c_void_p), ("kv_lens", C.c_void_p), ("q_starts", C.c_void_p),
                 ("page_table_len", C.c_size_t), ("kv_lens_len", C.c_size_t), ("q_starts_len", C.c_size_t),
-                ("n_seqs", C.c_uint32), ("table_stride", C.c_uint32), ("n_rows", C.c_uint32),
+                ("n_seqs", C.c_uint32), ("table_stride", C.c_uint32),
                 ("max_q_len", C.c_uint32), ("max_kv_len", C.c_uint32)]
 
 
 class _PagedAppend(C.Structure):
-    _fields_ = [("dtype", C.c_uint32), ("n_heads", C.c_uint32), ("q", C.c_void_p), ("k", C.c_void_p),
+    _fields_ = [("dtype", C.c_uint32), ("n_rows", C.c_uint32), ("n_heads", C.c_uint32), ("q", C.c_void_p), ("k", C.c_void_p),
                 ("v", C.c_void_p), ("q_out", C.c_void_p), ("q_len", C.c_size_t), ("k_len", C.c_size_t),
                 ("v_len", C.c_size_t), ("q_out_len", C.c_size_t), ("q_stride", C.c_int64), ("k_stride", C.c_int64),
                 ("v_stride", C.c_int64), ("q_out_stride", C.c_int64), ("cos_t", C.c_void_p), ("sin_t", C.c_void_p),
@@ -688,21 +689,26 @@ class _PagedAppend(C.Structure):
 
 
 class _PagedRead(C.Structure):
-    _fields_ = [("dtype", C.c_uint32), ("k", C.c_void_p), ("v", C.c_void_p), ("k_len", C.c_size_t),
+    _fields_ = [("dtype", C.c_uint32), ("n_rows", C.c_uint32), ("k", C.c_void_p), ("v", C.c_void_p), ("k_len", C.c_size_t),
                 ("v_len", C.c_size_t), ("k_stride", C.c_int64), ("v_stride", C.c_int64)]
 
 
 class _PagedAttention(C.Structure):
-    _fields_ = [("dtype", C.c_uint32), ("n_heads", C.c_uint32), ("q", C.c_void_p), ("out", C.c_void_p),
+    _fields_ = [("dtype", C.c_uint32), ("n_rows", C.c_uint32), ("n_heads", C.c_uint32), ("q", C.c_void_p), ("out", C.c_void_p),
                 ("q_len", C.c_size_t), ("out_len", C.c_size_t), ("q_stride", C.c_int64), ("out_stride", C.c_int64),
                 ("sinks", C.c_void_p), ("sinks_len", C.c_size_t), ("scale", C.c_float), ("window", C.c_uint32),
                 ("workspace", C.c_void_p), ("workspace_len", C.c_size_t)]
 
 
+# the same layouts for one pack() per call (a tenth of a field-by-field fill)
+_PAGED_APPEND = _struct.Struct("@IIIPPPPNNNNqqqqPPNIII")
+_PAGED_READ = _struct.Struct("@IIPPNNqq")
+_PAGED_ATTENTION = _struct.Struct("@IIIPPNNqqPNfIPN")
+
 _sig("rusty_hip_paged_kv_bytes", C.c_uint64, _u32, _u32, _u32, _u32, _u32)
 _sig("rusty_hip_paged_append", _i, _p, _p, _p, _p)
 _sig("rusty_hip_paged_read", _i, _p, _p, _p, _p)
-_sig("rusty_hip_paged_attention_workspace", C.c_uint64, _p, _p, _u32)
+_sig("rusty_hip_paged_attention_workspace", C.c_uint64, _p, _p, _u32, _u32)
 _sig("rusty_hip_paged_attention", _i, _p, _p, _p, _p)
 
 
@@ -711,11 +717,17 @@ def paged_kv_bytes(n_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
     return lib.rusty_hip_paged_kv_bytes(n_pages, page_size, n_kv_heads, head_dim, value_dim or head_dim)
 
 
+_DTYPE_NAMES = {}
+
+
 def _dev_bytes(t, what, dtype):
     """A contiguous device tensor's address and bytes."""
-    if str(t.dtype) != "torch." + dtype or not t.is_contiguous() or not t.is_cuda:
+    name = _DTYPE_NAMES.get(t.dtype)
+    if name is None:
+        name = _DTYPE_NAMES[t.dtype] = str(t.dtype)[len("torch."):]
+    if name != dtype or not t.is_contiguous() or not t.is_cuda:
         raise ValueError(f"{what}: a contiguous {dtype} tensor on the GPU is needed")
-    return t.data_ptr(), t.numel() * t.element_size()
+    return t.data_ptr(), t.nbytes
 
 
 class PagedKv:
@@ -725,12 +737,13 @@ class PagedKv:
     def __init__(self, k_pages, v_pages, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
                  value_dim: int | None = None):
         self.n_kv_heads, self.head_dim, self.value_dim = n_kv_heads, head_dim, value_dim or head_dim
-        self.device = k_pages.device
         k, k_len = _dev_bytes(k_pages, "k_pages", "uint8")
         v, v_len = _dev_bytes(v_pages, "v_pages", "uint8")
         need = paged_kv_bytes(n_pages, page_size, n_kv_heads, head_dim, self.value_dim)
-        if need == 0 or k_len < need or v_len < need or v_pages.device != self.device:
+        if need == 0 or k_len < need or v_len < need:
             raise ValueError("PagedKv: sizes that are not taken, or pages shorter than paged_kv_bytes")
+        if k_pages.get_device() != 0 or v_pages.get_device() != 0:
+            raise ValueError("PagedKv: pages on the library's device (device 0) are needed")
         self._c = _PagedKv(k, v, k_len, v_len, n_pages, page_size, n_kv_heads, head_dim, self.value_dim)
         self._ref = C.addressof(self._c)
         self._keep = (k_pages, v_pages)
@@ -746,45 +759,50 @@ class PagedBatch:
         n, stride = page_table.shape
         if n == 0 or tuple(kv_lens.shape) != (n,) or tuple(q_starts.shape) != (n + 1,):
             raise ValueError("PagedBatch: page_table [n][stride], kv_lens [n] and q_starts [n + 1] are needed")
-        self.device = page_table.device
-        if kv_lens.device != self.device or q_starts.device != self.device:
-            raise ValueError("PagedBatch: tensors of one device are needed")
         t, t_len = _dev_bytes(page_table, "page_table", "int32")
         l, l_len = _dev_bytes(kv_lens, "kv_lens", "int32")
         q, q_len = _dev_bytes(q_starts, "q_starts", "int32")
-        self._c = _PagedBatch(t, l, q, t_len, l_len, q_len, n, stride, 0, max_q_len, max_kv_len)
+        if page_table.get_device() != 0 or kv_lens.get_device() != 0 or q_starts.get_device() != 0:
+            raise ValueError("PagedBatch: tensors on the library's device (device 0) are needed")
+        self._c = _PagedBatch(t, l, q, t_len, l_len, q_len, n, stride, max_q_len, max_kv_len)
         self._ref = C.addressof(self._c)
         self._keep = (page_table, kv_lens, q_starts)
 
 
-def _rows(kv, t, what, dtype, n, heads, dim):
+def _rows(t, what, dtype, n, heads, dim):
     """Address, bytes and row stride of a [rows][heads][dim] device tensor."""
-    if t.dtype != dtype or t.device != kv.device or tuple(t.shape) != (n, heads, dim):
-        raise ValueError(f"{what}: a {dtype} tensor [{n}][{heads}][{dim}] on {kv.device} is needed")
+    if t.dtype is not dtype or t.shape != (n, heads, dim) or t.get_device() != 0:
+        raise ValueError(f"{what}: a {dtype} tensor [{n}][{heads}][{dim}] on device 0 is needed")
     row, head, one = t.stride()
-    if (one != 1 and dim > 1) or (head != dim and heads > 1):
+    if one != 1 or (head != dim and heads > 1):
         raise ValueError(f"{what}: rows without gaps are needed")
-    if n <= 1:
+    if n == 1:
         row = heads * dim
     return t.data_ptr(), ((n - 1) * row + heads * dim) * t.element_size(), row
 
 
-_PAGED_DTYPE = {"torch.float32": 0, "torch.bfloat16": 1}
+_PAGED_DTYPE = {}
+_current_stream = None
 
 
-def _paged_call(kv, batch, t, stream):
-    """dtype code and rows of the row tensor t, and the stream: the caller's, or
-    torch's current one on the cache's device."""
-    if batch.device != kv.device or kv.device.index not in (0, None):
-        raise ValueError("paged cache: one device, the library's (device 0), is needed")
-    code = _PAGED_DTYPE.get(str(t.dtype))
+def _paged_call(t, stream):
+    """dtype code of the row tensor t, and the stream: the caller's, or torch's
+    current one on device 0."""
+    global _current_stream
+    code = _PAGED_DTYPE.get(t.dtype)
     if code is None:
-        raise ValueError("paged cache: float32 or bfloat16 rows are needed")
+        code = {"torch.float32": 0, "torch.bfloat16": 1}.get(str(t.dtype))
+        if code is None:
+            raise ValueError("paged cache: float32 or bfloat16 rows are needed")
+        _PAGED_DTYPE[t.dtype] = code
     if stream is None:
-        import torch
-        stream = torch.cuda.current_stream(kv.device).cuda_stream
-    batch._c.n_rows = t.shape[0]
-    return code, t.shape[0], stream
+        if _current_stream is None:
+            import torch
+            # the handle alone, where torch offers it (0.1 us, 1.3 with the stream object)
+            _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+                lambda index: torch.cuda.current_stream(index).cuda_stream)
+        stream = _current_stream(0)
+    return code, stream
 
 
 def paged_append_dev(kv: PagedKv, batch: PagedBatch, k, v, cos, sin, q=None, q_out=None, neox: bool = False,
@@ -792,27 +810,29 @@ def paged_append_dev(kv: PagedKv, batch: PagedBatch, k, v, cos, sin, q=None, q_o
     """rusty_hip_paged_append: rotates q (into q_out, which may be q) and k by
     the f32 tables cos / sin [max_pos][rot_dim / 2], and quantizes k and v into
     their pages.  Rows are [rows][heads][dim] device tensors, float32 or
-    bfloat16, of any row stride.  Asynchronous on `stream`."""
+    bfloat16, of any row stride that is a multiple of four.  Asynchronous on
+    `stream` (a HIP stream handle; None: torch's current stream)."""
     if not enabled():
         return False
-    code, n, stream = _paged_call(kv, batch, k, stream)
-    t = k.dtype
-    a = _PagedAppend(dtype=code, neox=1 if neox else 0)
-    a.k, a.k_len, a.k_stride = _rows(kv, k, "k", t, n, kv.n_kv_heads, kv.head_dim)
-    a.v, a.v_len, a.v_stride = _rows(kv, v, "v", t, n, kv.n_kv_heads, kv.value_dim)
+    code, stream = _paged_call(k, stream)
+    t, n = k.dtype, k.shape[0]
+    k_at, k_len, k_row = _rows(k, "k", t, n, kv.n_kv_heads, kv.head_dim)
+    v_at, v_len, v_row = _rows(v, "v", t, n, kv.n_kv_heads, kv.value_dim)
+    heads = q_at = q_len = q_row = o_at = o_len = o_row = 0
     if q is not None:
-        heads = q.shape[1]
         if q_out is None:
             raise ValueError("paged_append_dev: q needs q_out (which may be q)")
-        a.n_heads = heads
-        a.q, a.q_len, a.q_stride = _rows(kv, q, "q", t, n, heads, kv.head_dim)
-        a.q_out, a.q_out_len, a.q_out_stride = _rows(kv, q_out, "q_out", t, n, heads, kv.head_dim)
-    if cos.shape != sin.shape or cos.device != kv.device or sin.device != kv.device:
-        raise ValueError("paged_append_dev: cos and sin [max_pos][rot_dim / 2] on the cache's device are needed")
-    a.cos_t, a.table_len = _dev_bytes(cos, "cos", "float32")
-    a.sin_t, _ = _dev_bytes(sin, "sin", "float32")
-    a.max_pos, a.rot_dim = cos.shape[0], 2 * cos.shape[1]
-    return lib.rusty_hip_paged_append(kv._ref, batch._ref, C.addressof(a), stream) == 1
+        heads = q.shape[1]
+        q_at, q_len, q_row = _rows(q, "q", t, n, heads, kv.head_dim)
+        o_at, o_len, o_row = _rows(q_out, "q_out", t, n, heads, kv.head_dim)
+    if cos.shape != sin.shape or cos.get_device() != 0 or sin.get_device() != 0:
+        raise ValueError("paged_append_dev: cos and sin [max_pos][rot_dim / 2] on device 0 are needed")
+    cos_at, table_len = _dev_bytes(cos, "cos", "float32")
+    sin_at, _ = _dev_bytes(sin, "sin", "float32")
+    max_pos, half = cos.shape
+    return lib.rusty_hip_paged_append(kv._ref, batch._ref, _PAGED_APPEND.pack(
+        code, n, heads, q_at, k_at, v_at, o_at, q_len, k_len, v_len, o_len, q_row, k_row, v_row, o_row, cos_at, sin_at,
+        table_len, max_pos, 2 * half, 1 if neox else 0), stream) == 1
 
 
 def paged_read_dev(kv: PagedKv, batch: PagedBatch, k_out=None, v_out=None, stream: int | None = None) -> bool:
@@ -822,19 +842,20 @@ def paged_read_dev(kv: PagedKv, batch: PagedBatch, k_out=None, v_out=None, strea
     first = k_out if k_out is not None else v_out
     if first is None:
         raise ValueError("paged_read_dev: k_out or v_out is needed")
-    code, n, stream = _paged_call(kv, batch, first, stream)
-    a = _PagedRead(dtype=code)
+    code, stream = _paged_call(first, stream)
+    t, n = first.dtype, first.shape[0]
+    k_at = k_len = k_row = v_at = v_len = v_row = 0
     if k_out is not None:
-        a.k, a.k_len, a.k_stride = _rows(kv, k_out, "k_out", first.dtype, n, kv.n_kv_heads, kv.head_dim)
+        k_at, k_len, k_row = _rows(k_out, "k_out", t, n, kv.n_kv_heads, kv.head_dim)
     if v_out is not None:
-        a.v, a.v_len, a.v_stride = _rows(kv, v_out, "v_out", first.dtype, n, kv.n_kv_heads, kv.value_dim)
-    return lib.rusty_hip_paged_read(kv._ref, batch._ref, C.addressof(a), stream) == 1
+        v_at, v_len, v_row = _rows(v_out, "v_out", t, n, kv.n_kv_heads, kv.value_dim)
+    return lib.rusty_hip_paged_read(kv._ref, batch._ref, _PAGED_READ.pack(
+        code, n, k_at, v_at, k_len, v_len, k_row, v_row), stream) == 1
 
 
 def paged_attention_workspace(kv: PagedKv, batch: PagedBatch, n_rows: int, n_heads: int) -> int:
     """Workspace bytes of paged_attention_dev for n_rows rows of n_heads query heads."""
-    batch._c.n_rows = n_rows
-    return lib.rusty_hip_paged_attention_workspace(kv._ref, batch._ref, n_heads)
+    return lib.rusty_hip_paged_attention_workspace(kv._ref, batch._ref, n_rows, n_heads)
 
 
 def paged_attention_dev(kv: PagedKv, batch: PagedBatch, q, out, scale: float, workspace=None, sinks=None,
@@ -844,17 +865,18 @@ def paged_attention_dev(kv: PagedKv, batch: PagedBatch, q, out, scale: float, wo
     paged_attention_workspace bytes, used by one call at a time."""
     if not enabled():
         return False
-    code, n, stream = _paged_call(kv, batch, q, stream)
-    heads = q.shape[1]
-    a = _PagedAttention(dtype=code, n_heads=heads, scale=scale, window=window)
-    a.q, a.q_len, a.q_stride = _rows(kv, q, "q", q.dtype, n, heads, kv.head_dim)
-    a.out, a.out_len, a.out_stride = _rows(kv, out, "out", q.dtype, n, heads, kv.value_dim)
+    code, stream = _paged_call(q, stream)
+    n, heads, _ = q.shape
+    q_at, q_len, q_row = _rows(q, "q", q.dtype, n, heads, kv.head_dim)
+    o_at, o_len, o_row = _rows(out, "out", q.dtype, n, heads, kv.value_dim)
+    s_at = s_len = w_at = w_len = 0
     if sinks is not None:
-        if sinks.device != kv.device:
-            raise ValueError("paged_attention_dev: sinks on the cache's device are needed")
-        a.sinks, a.sinks_len = _dev_bytes(sinks, "sinks", "float32")
+        if sinks.get_device() != 0:
+            raise ValueError("paged_attention_dev: sinks on device 0 are needed")
+        s_at, s_len = _dev_bytes(sinks, "sinks", "float32")
     if workspace is not None:
-        if workspace.device != kv.device:
-            raise ValueError("paged_attention_dev: a workspace on the cache's device is needed")
-        a.workspace, a.workspace_len = _dev_bytes(workspace, "workspace", "uint8")
-    return lib.rusty_hip_paged_attention(kv._ref, batch._ref, C.addressof(a), stream) == 1
+        if workspace.get_device() != 0:
+            raise ValueError("paged_attention_dev: a workspace on device 0 is needed")
+        w_at, w_len = _dev_bytes(workspace, "workspace", "uint8")
+    return lib.rusty_hip_paged_attention(kv._ref, batch._ref, _PAGED_ATTENTION.pack(
+        code, n, heads, q_at, o_at, q_len, o_len, q_row, o_row, s_at, s_len, scale, window, w_at, w_len), stream) == 1

@@ -29,10 +29,21 @@ def test_large_pool_bytes_do_not_wrap():
 def test_struct_layouts():
     """Offsets of the C structs (include/rusty_hip.h) on a 64-bit host."""
     assert C.sizeof(hip._PagedKv) == 56 and hip._PagedKv.n_pages.offset == 32
-    assert C.sizeof(hip._PagedBatch) == 72 and hip._PagedBatch.n_seqs.offset == 48
-    assert hip._PagedAppend.cos_t.offset == 104 and C.sizeof(hip._PagedAppend) == 144
+    assert C.sizeof(hip._PagedBatch) == 64 and hip._PagedBatch.n_seqs.offset == 48
+    assert hip._PagedAppend.cos_t.offset == 112 and C.sizeof(hip._PagedAppend) == 152
     assert hip._PagedRead.k.offset == 8 and C.sizeof(hip._PagedRead) == 56
-    assert hip._PagedAttention.scale.offset == 72 and C.sizeof(hip._PagedAttention) == 96
+    assert hip._PagedAttention.scale.offset == 80 and C.sizeof(hip._PagedAttention) == 104
+
+
+@pytest.mark.parametrize("packed,fields", [("_PAGED_APPEND", "_PagedAppend"), ("_PAGED_READ", "_PagedRead"),
+                                           ("_PAGED_ATTENTION", "_PagedAttention")])
+def test_packed_rows_are_the_struct(packed, fields):
+    """pack() writes every field where the struct has it."""
+    fmt, struct = getattr(hip, packed), getattr(hip, fields)
+    values = [0.5 if t is C.c_float else 3 + i for i, (_, t) in enumerate(struct._fields_)]
+    data = fmt.pack(*values).ljust(C.sizeof(struct), b"\0")
+    got = struct.from_buffer_copy(data)
+    assert [getattr(got, name) for name, _ in struct._fields_] == values
 
 
 class _Call:
@@ -42,12 +53,12 @@ class _Call:
     def __init__(self):
         size = hip.paged_kv_bytes(9, 32, 2, 64)
         self.kv = hip._PagedKv(4096, 8192, size, size, 9, 32, 2, 64, 64)
-        self.batch = hip._PagedBatch(4096, 4096, 4096, 2 * 5 * 4, 8, 12, 2, 5, 3, 2, 100)
+        self.batch = hip._PagedBatch(4096, 4096, 4096, 2 * 5 * 4, 8, 12, 2, 5, 2, 100)
         row = 2 * 64 * 4
-        self.append = hip._PagedAppend(0, 4, 4096, 4096, 4096, 4096, 6 * row, 3 * row, 3 * row, 6 * row, 256, 128, 128,
+        self.append = hip._PagedAppend(0, 3, 4, 4096, 4096, 4096, 4096, 6 * row, 3 * row, 3 * row, 6 * row, 256, 128, 128,
                                        256, 4096, 4096, 100 * 32 * 4, 100, 64, 0)
-        self.read = hip._PagedRead(0, 4096, 4096, 3 * row, 3 * row, 128, 128)
-        self.attn = hip._PagedAttention(0, 4, 4096, 4096, 6 * row, 6 * row, 256, 256, None, 0, 0.125, 0, 4096, 1 << 30)
+        self.read = hip._PagedRead(0, 3, 4096, 4096, 3 * row, 3 * row, 128, 128)
+        self.attn = hip._PagedAttention(0, 3, 4, 4096, 4096, 6 * row, 6 * row, 256, 256, None, 0, 0.125, 0, 4096, 1 << 30)
 
     def all(self):
         L, r = hip.lib, C.addressof
@@ -61,8 +72,8 @@ class _Call:
     ("kv", "n_pages", 0), ("kv", "page_size", 24), ("kv", "n_kv_heads", 0), ("kv", "head_dim", 260),
     ("kv", "value_dim", 12), ("batch", "page_table", None), ("batch", "kv_lens", None), ("batch", "q_starts", None),
     ("batch", "page_table_len", 39), ("batch", "kv_lens_len", 7), ("batch", "q_starts_len", 8), ("batch", "n_seqs", 0),
-    ("batch", "table_stride", 0), ("batch", "n_rows", 0), ("batch", "max_q_len", 0), ("batch", "kv_lens", 4098),
-    ("batch", "n_seqs", 1 << 25), ("batch", "n_rows", 1 << 25), ("batch", "table_stride", 1 << 25),
+    ("batch", "table_stride", 0), ("batch", "max_q_len", 0), ("batch", "kv_lens", 4098),
+    ("batch", "n_seqs", 1 << 25), ("batch", "table_stride", 1 << 25),
 ])
 def test_refused_by_every_call(struct, field, value):
     c = _Call()
@@ -71,6 +82,8 @@ def test_refused_by_every_call(struct, field, value):
 
 
 @pytest.mark.parametrize("struct,at,field,value", [
+    ("append", 0, "n_rows", 0), ("append", 0, "n_rows", 1 << 25), ("append", 0, "n_rows", 4), ("read", 1, "n_rows", 0),
+    ("read", 1, "n_rows", 4), ("attn", 2, "n_rows", 0), ("attn", 2, "n_rows", 4),
     ("append", 0, "dtype", 2), ("append", 0, "k", None), ("append", 0, "v", None), ("append", 0, "q_out", None),
     ("append", 0, "n_heads", 3), ("append", 0, "n_heads", 0), ("append", 0, "q_len", 3071), ("append", 0, "k_len", 10),
     ("append", 0, "k_stride", 126), ("append", 0, "k_stride", 64), ("append", 0, "v_stride", -128),
@@ -108,7 +121,7 @@ def test_without_a_gpu_nothing_is_handled():
 
 def test_workspace_grows_with_the_split():
     c = _Call()
-    f = lambda: hip.lib.rusty_hip_paged_attention_workspace(C.addressof(c.kv), C.addressof(c.batch), 4)  # noqa: E731
+    f = lambda: hip.lib.rusty_hip_paged_attention_workspace(C.addressof(c.kv), C.addressof(c.batch), 3, 4)  # noqa: E731
     c.batch.max_kv_len = 16
     small = f()
     c.batch.max_kv_len = 100000
