@@ -578,7 +578,8 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : G == 4 ? (R == 4 && !F32 ? 3 :
 // are 32x32x16 products K q^T, so that a lane holds one row's p against 16 tokens of
 // each 32 and feeds them to V^T p without leaving its registers: V's tokens lie in
 // LDS in the order (quads 0 2 1 3 of 16) in which the scores come.  LDS holds two
-// steps: one is unpacked while the other is worked on, with one barrier per step.
+// steps: one is unpacked while the other is worked on, with one barrier per step (one
+// step of f32 rows from 128 channels on, so that two workgroups fit a CU).
 // For f32 rows q, K, p and V are two halves each and the products of their small
 // parts are left out (2^-22 of the result).
 //
@@ -586,8 +587,8 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : G == 4 ? (R == 4 && !F32 ? 3 :
 // instructions (32 of them exponentials at a quarter of the rate), its share of the
 // unpacking 75, against 32 products of 32 clocks.
 template <int G, bool F32, int W>
-__global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void paged_attn_tile_kernel(PagedDev P, PagedAttn A) {
-    constexpr int DV = 32 * G, N = F32 ? 2 : 1, NB = G == 8 && F32 ? 1 : 2, SETS = W == 8 ? 1 : 2;
+__global__ __launch_bounds__(64 * W, G == 8 ? 1 : 2) void paged_attn_tile_kernel(PagedDev P, PagedAttn A) {
+    constexpr int DV = 32 * G, N = F32 ? 2 : 1, NB = G >= 4 && F32 ? 1 : 2, SETS = W == 8 ? 1 : 2;
     __shared__ half8v s_k[NB][N][64 * DV / 8], s_v[NB][N][DV * 64 / 8];
     __shared__ uint32_t s_most[2][4], s_page[2][4];
     __shared__ uint8_t s_bad[2][64][G];
@@ -993,14 +994,20 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void paged_attn_tile_kernel
     l *= 1.0f / 64.0f;
     if (!on) return;
     const float unit = ldexpf(1.0f, -E - 6);
-    const int hd = kvh * A.kv_mul + h0 + my_head;
+    // the arguments used from here on are read here: kept through the loop, they
+    // pushed others out of the scalar registers (25 lane reads per step)
+    typedef __attribute__((address_space(4))) const uint8_t kernarg_t;
+    kernarg_t *args = (kernarg_t *)__builtin_amdgcn_kernarg_segment_ptr() + sizeof(PagedDev);
+    asm volatile("" : "+s"(args));
+    const auto &B = *(__attribute__((address_space(4))) const PagedAttn *)args;
+    const int hd = kvh * B.kv_mul + h0 + my_head;
     const int64_t token = row0 + tok + my_tok;
     const bool none = m == -__builtin_inff();
-    if (A.n_splits > 1) {
-        const int64_t to = ((int64_t)split * P.n_tokens + token) * A.n_heads + hd;
+    if (B.n_splits > 1) {
+        const int64_t to = ((int64_t)split * P.n_tokens + token) * B.n_heads + hd;
         if (half == 0) {
-            A.ml[to * 2] = m;
-            A.ml[to * 2 + 1] = l;
+            B.ml[to * 2] = m;
+            B.ml[to * 2 + 1] = l;
         }
         if (!none)
 #pragma unroll
@@ -1008,13 +1015,13 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void paged_attn_tile_kernel
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
                     const float y[4] = {acc[g][i] * unit, acc[g][i + 1] * unit, acc[g][i + 2] * unit, acc[g][i + 3] * unit};
-                    row_store4(A.part + to * DV + 32 * g + 2 * i + 4 * half, y);
+                    row_store4(B.part + to * DV + 32 * g + 2 * i + 4 * half, y);
                 }
         return;
     }
     float f = none ? 0.0f : unit / l;
-    if (A.sinks && !none) {
-        const float sink = A.sinks[hd] * 1.44269504f, top = fmaxf(m, sink), a = __builtin_amdgcn_exp2f(m - top);
+    if (B.sinks && !none) {
+        const float sink = B.sinks[hd] * 1.44269504f, top = fmaxf(m, sink), a = __builtin_amdgcn_exp2f(m - top);
         f = unit * a / fmaf(l, a, __builtin_amdgcn_exp2f(sink - top));
     }
 #pragma unroll
@@ -1025,11 +1032,11 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void paged_attn_tile_kernel
             if (ch >= P.vd) continue;
             const float y[4] = {none ? 0.0f : acc[g][i] * f, none ? 0.0f : acc[g][i + 1] * f,
                                 none ? 0.0f : acc[g][i + 2] * f, none ? 0.0f : acc[g][i + 3] * f};
-            const int64_t to = token * A.o_stride + (int64_t)hd * P.vd + ch;
+            const int64_t to = token * B.o_stride + (int64_t)hd * P.vd + ch;
             if (F32)
-                row_store4((float *)A.out + to, y);
+                row_store4((float *)B.out + to, y);
             else
-                row_store4((uint16_t *)A.out + to, y);
+                row_store4((uint16_t *)B.out + to, y);
         }
 }
 
