@@ -509,11 +509,54 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : G == 4 ? (R == 4 && !F32 ? 3 :
         load_v((more ? k + 1 : k) & 15);
     }
 
-    // the lanes' results through LDS, and the waves' joined
+    // a row's lanes hold parts of its sum
     if (NT >= 4) l += paged_dpp<0x124>(l);
     if (NT >= 2) l += paged_dpp<0x128>(l);
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
+    if (W == 1) {  // the wave's lanes hold whole results: four channels of a row each
+        if (col >= R || !on) return;
+        const int hd = kvh * A.kv_mul + h0 + my_head;
+        const int64_t token = row0 + my_tok;
+        const bool none = m == -__builtin_inff();
+        const float one = ldexpf(1.0f, -(int)E);
+        if (A.n_splits > 1) {
+            const int64_t to = ((int64_t)split * P.n_tokens + token) * A.n_heads + hd;
+            if (quad == 0) {
+                A.ml[to * 2] = m;
+                A.ml[to * 2 + 1] = l * one;
+            }
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float y[4] = {acc[g][h][0] * one, acc[g][h][1] * one, acc[g][h][2] * one, acc[g][h][3] * one};
+                    if (!none) row_store4(A.part + to * DV + 32 * g + 16 * h + 4 * quad, y);
+                }
+            return;
+        }
+        float f = none ? 0.0f : 1.0f / l;
+        if (A.sinks && !none) {
+            const float sink = A.sinks[hd] * 1.44269504f, top = fmaxf(m, sink), a = __builtin_amdgcn_exp2f(m - top);
+            f = a * one / fmaf(l * one, a, __builtin_amdgcn_exp2f(sink - top));
+        }
+#pragma unroll
+        for (int g = 0; g < G; g++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int ch = 32 * g + 16 * h + 4 * quad;
+                if (ch >= P.vd) continue;
+                float y[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) y[j] = none ? 0.0f : acc[g][h][j] * f;
+                const int64_t to = token * A.o_stride + (int64_t)hd * P.vd + ch;
+                if (F32)
+                    row_store4((float *)A.out + to, y);
+                else
+                    row_store4((uint16_t *)A.out + to, y);
+            }
+        return;
+    }
     const float unit = ldexpf(1.0f, -(int)E);
     __shared__ float s_acc[W][R][DV + 4];
     __shared__ float s_m[W][R], s_l[W][R];
