@@ -1143,59 +1143,72 @@ __global__ __launch_bounds__(256) void paged_attn_join_rows_kernel(PagedDev P, P
 }
 
 // The same for the rows of larger tiles, of which there are many with few splits:
-// one wave per (row, query head).
+// one wave per (row, four query heads), their loads in flight together.
 template <int G, bool F32>
 __global__ __launch_bounds__(256) void paged_attn_join_tiles_kernel(PagedDev P, PagedAttn A) {
-    constexpr int DV = 32 * G, N = DV / 64;
+    constexpr int DV = 32 * G, N = DV / 64, H = 4;
     const int lane = threadIdx.x & 63;
     const int64_t rows = (int64_t)P.n_tokens * A.n_heads, w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (w >= rows) return;
-    const int token = (int)(w / A.n_heads), hd = (int)(w - (int64_t)token * A.n_heads);
+    const int groups = (A.n_heads + H - 1) / H;
+    const int token = (int)(w / groups), hd = (int)(w - (int64_t)token * groups) * H;
+    if (token >= P.n_tokens) return;
     int seq, a, b;
     // rows of no session stay as they are
     if (!paged_session(P, token, &seq, &a, &b) || (A.both && b - a <= A.short_q)) return;
-    float top = -__builtin_inff();
-    for (int s = lane; s < A.n_splits; s += 64) top = fmaxf(top, A.ml[(s * rows + w) * 2]);
-    top = wave_max(top);
-    const bool none = top == -__builtin_inff();
-    float base = none ? 0.0f : top, sum = 0.0f;
-    if (A.sinks) {
-        const float sink = A.sinks[hd] * 1.44269504f;
-        base = none ? sink : fmaxf(base, sink);
-        sum = __builtin_amdgcn_exp2f(sink - base);
+    int64_t at[H];
+    float top[H], base[H], sum[H], o[H][N];
+#pragma unroll
+    for (int h = 0; h < H; h++) {
+        at[h] = (int64_t)token * A.n_heads + (hd + h < A.n_heads ? hd + h : hd);
+        top[h] = -__builtin_inff();
     }
-    float o[N] = {};
-    for (int s = 0; s < A.n_splits; s += 4) {
-        float x[4][N], m[4], l[4];
+    for (int s = 0; s < A.n_splits; s++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int64_t at = (s + j < A.n_splits ? s + j : s) * rows + w;
-            m[j] = A.ml[at * 2];
-            l[j] = A.ml[at * 2 + 1];
+        for (int h = 0; h < H; h++) top[h] = fmaxf(top[h], A.ml[(s * rows + at[h]) * 2]);
 #pragma unroll
-            for (int n = 0; n < N; n++) x[j][n] = A.part[at * DV + lane + 64 * n];
+    for (int h = 0; h < H; h++) {
+        base[h] = top[h] == -__builtin_inff() ? 0.0f : top[h];
+        sum[h] = 0.0f;
+        if (A.sinks) {
+            const float sink = A.sinks[hd + h < A.n_heads ? hd + h : hd] * 1.44269504f;
+            base[h] = top[h] == -__builtin_inff() ? sink : fmaxf(top[h], sink);
+            sum[h] = __builtin_amdgcn_exp2f(sink - base[h]);
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int n = 0; n < N; n++) o[h][n] = 0.0f;
+    }
+    for (int s = 0; s < A.n_splits; s++) {
+        float x[H][N], m[H], l[H];
+#pragma unroll
+        for (int h = 0; h < H; h++) {
+            m[h] = A.ml[(s * rows + at[h]) * 2];
+            l[h] = A.ml[(s * rows + at[h]) * 2 + 1];
+#pragma unroll
+            for (int n = 0; n < N; n++) x[h][n] = A.part[(s * rows + at[h]) * DV + lane + 64 * n];
+        }
+#pragma unroll
+        for (int h = 0; h < H; h++) {
             // a split without keys wrote no sums
-            const bool has = s + j < A.n_splits && m[j] != -__builtin_inff();
-            const float f = has ? __builtin_amdgcn_exp2f(m[j] - base) : 0.0f;
-            sum = has ? fmaf(f, l[j], sum) : sum;
+            const bool has = m[h] != -__builtin_inff();
+            const float f = has ? __builtin_amdgcn_exp2f(m[h] - base[h]) : 0.0f;
+            sum[h] = has ? fmaf(f, l[h], sum[h]) : sum[h];
 #pragma unroll
-            for (int n = 0; n < N; n++) o[n] = has ? fmaf(f, x[j][n], o[n]) : o[n];
+            for (int n = 0; n < N; n++) o[h][n] = has ? fmaf(f, x[h][n], o[h][n]) : o[h][n];
         }
     }
 #pragma unroll
-    for (int n = 0; n < N; n++) {
-        const int ch = lane + 64 * n;
-        if (ch >= P.vd) continue;
-        const float y = none ? 0.0f : o[n] / sum;
-        const int64_t to = token * A.o_stride + (int64_t)hd * P.vd + ch;
-        if (F32)
-            ((float *)A.out)[to] = y;
-        else
-            ((uint16_t *)A.out)[to] = f32_to_bf16(y);
-    }
+    for (int h = 0; h < H; h++)
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const int ch = lane + 64 * n;
+            if (ch >= P.vd || hd + h >= A.n_heads) continue;
+            const float y = top[h] == -__builtin_inff() ? 0.0f : o[h][n] / sum[h];
+            const int64_t to = token * A.o_stride + (int64_t)(hd + h) * P.vd + ch;
+            if (F32)
+                ((float *)A.out)[to] = y;
+            else
+                ((uint16_t *)A.out)[to] = f32_to_bf16(y);
+        }
 }
 
 }  // namespace rh

@@ -4524,14 +4524,16 @@ static PagedPlan paged_plan(const PagedDev &P, uint32_t n_heads, uint32_t max_q,
         p.waves = P.hd > 64 || P.vd > 64 || (int64_t)max_q * chunk <= 128 ? 4 : 8;
         p.tok_tile = 32 * p.waves / chunk;
         p.tiles = P.n_tokens / p.tok_tile + (int64_t)P.n_seqs;
-        // eight waves per CU, of 4 steps or more each
+        // splits of 4 steps or more, as long as eight waves per CU take to share all steps:
+        // the shorter last ones fill the gaps
         const int64_t steps = steps_of(p.tok_tile), items = (P.n_tokens + p.tok_tile - 1) / p.tok_tile * p.heads_y;
-        int64_t n = 256 * 8 / p.waves / items;
-        if (n > (steps + 3) / 4) n = (steps + 3) / 4;
-        if (n < 1) n = 1;
-        if (n > 256) n = 256;
-        p.tile_splits = (int)n;
-        p.tile_steps = (int)((steps + n - 1) / n);
+        const int64_t slots = 256 * 8 / p.waves;
+        int64_t per = (steps * items + slots - 1) / slots;
+        if (per < 4) per = 4;
+        if ((steps + per - 1) / per > 256) per = (steps + 255) / 256;
+        if (per > steps) per = steps;
+        p.tile_splits = (int)((steps + per - 1) / per);
+        p.tile_steps = (int)per;
     }
     return p;
 }
@@ -4573,7 +4575,7 @@ static void paged_attn_launch(const PagedDev &P, PagedAttn A, const PagedPlan &p
             paged_attn_tile_kernel<G, F32, 8><<<grid, 512, 0, s>>>(P, A);
         if (p.tile_splits > 1)
             paged_attn_join_tiles_kernel<G, F32>
-                <<<(unsigned)(((int64_t)P.n_tokens * A.n_heads + 3) / 4), 256, 0, s>>>(P, A);
+                <<<(unsigned)(((int64_t)P.n_tokens * ((A.n_heads + 3) / 4) + 3) / 4), 256, 0, s>>>(P, A);
     }
     if (p.short_q) {
         tiles_of(p.short_q, p.splits, p.steps, 1 << 8);
