@@ -613,25 +613,28 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : G == 4 ? (R == 4 && !F32 ? 3 :
     }
 }
 
-// Prompts and longer chunks: tiles of up to 32 W rows (tokens x query heads of one
-// kv head), 32 per wave, whose keys and values the workgroup unpacks once per
-// 64 cached tokens into LDS: K as halves [token][channel], V as halves
-// [channel][token] times 2^E, where E keeps the largest |d| of the steps so far at
-// 2^12.  Of 8 waves four unpack keys and four values, of 4 each does both.  Scores
-// are 32x32x16 products K q^T, so that a lane holds one row's p against 16 tokens of
-// each 32 and feeds them to V^T p without leaving its registers: V's tokens lie in
-// LDS in the order (quads 0 2 1 3 of 16) in which the scores come.  LDS holds two
-// steps: one is unpacked while the other is worked on, with one barrier per step (one
-// step of f32 rows from 128 channels on, so that two workgroups fit a CU).
-// For f32 rows q, K, p and V are two halves each and the products of their small
-// parts are left out (2^-22 of the result).
+// Prompts and longer chunks: tiles of up to 128 rows (tokens x query heads of one kv
+// head), 32 per wave, whose keys and values the workgroup unpacks once per 64 cached
+// tokens into LDS: K as halves [token][channel], V as halves [channel][token] times
+// 2^E, where E keeps the largest |d| of the steps so far at 2^12.  Scores are
+// 32x32x16 products K q^T, so that a lane holds one row's p against 16 tokens of each
+// 32 and feeds them to V^T p without leaving its registers: V's tokens lie in LDS in
+// the order (quads 0 2 1 3 of 16) in which the scores come.  LDS holds two steps: one
+// is unpacked while the other is worked on, with one barrier per step (one step of f32
+// rows from 128 channels on, so that two workgroups fit a CU).  For f32 rows q, K, p
+// and V are two halves each and the products of their small parts are left out (2^-22
+// of the result).
 //
-// VALU issue bounds it for bf16 rows: a wave's 32 x 64 scores cost about 150
-// instructions (32 of them exponentials at a quarter of the rate), its share of the
-// unpacking 75, against 32 products of 32 clocks.
-template <int G, bool F32, int W>
-__global__ __launch_bounds__(64 * W, G == 8 ? 1 : 2) void paged_attn_tile_kernel(PagedDev P, PagedAttn A) {
-    constexpr int DV = 32 * G, N = F32 ? 2 : 1, NB = G >= 4 && F32 ? 1 : 2, SETS = W == 8 ? 1 : 2;
+// What bounds it: a wave's step of 32 rows x 64 tokens x 128 channels (bf16) is 32
+// products of 32 clocks and about 370 VALU instructions, 147 of them for the softmax
+// (32 exponentials at a quarter of the rate) and 142 for unpacking, and the two add up
+// also across the waves of a SIMD: 2900 clocks by the counters' busy cycles, 3020
+// measured.  Eight waves that share the unpacking (half per wave) waited longer at the
+// barrier than that saved: 92 us for a mixed step of 64-channel heads, 84 with four.
+__host__ __device__ constexpr int paged_tiles_per_cu(int G) { return G == 8 ? 1 : G == 4 ? 2 : 3; }
+template <int G, bool F32>
+__global__ __launch_bounds__(256, paged_tiles_per_cu(G)) void paged_attn_tile_kernel(PagedDev P, PagedAttn A) {
+    constexpr int DV = 32 * G, N = F32 ? 2 : 1, NB = G >= 4 && F32 ? 1 : 2;
     __shared__ half8v s_k[NB][N][64 * DV / 8], s_v[NB][N][DV * 64 / 8];
     __shared__ uint32_t s_most[2][4], s_page[2][4];
     __shared__ uint8_t s_bad[2][64][G];
@@ -643,8 +646,7 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : 2) void paged_attn_tile_kernel
         return r * (DV / 8) + (c ^ h);
     };
     auto v_at = [](int r, int c) __attribute__((always_inline)) { return r * 8 + (c ^ ((r >> 1) & 7)); };
-    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), w4 = wave & 3;
-    const bool do_k = W == 4 || wave < 4, do_v = W == 4 || wave >= 4;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int heads_y = P.n_kv * A.n_chunk, n_tiles = (int)(gridDim.x / (uint32_t)heads_y);
     const int x = (int)(blockIdx.x / (uint32_t)heads_y), head_y = (int)blockIdx.x - x * heads_y;
@@ -664,12 +666,12 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : 2) void paged_attn_tile_kernel
     const int s_hi = s_lo + per < rg.steps ? s_lo + per : rg.steps;
     const int64_t head_off = (int64_t)kvh * P.block;
 
-    // a wave unpacks the 16-token tile w4 of each step; lane j looks up where it lies
+    // a wave unpacks the 16-token tile wave of each step; lane j looks up where it lies
     // in step j of the next 64
     uint64_t where = 0, ok = 0;
     int off_tok = 0;
     auto look = [&](int s) __attribute__((always_inline)) {
-        const int t = rg.first + (s + lane) * 64 + 16 * w4;
+        const int t = rg.first + (s + lane) * 64 + 16 * wave;
         const bool in = s + lane < s_hi && t < rg.hi;
         int off = 0;
         const int page = in ? paged_page(P, seq, t, &off) : -1;
@@ -677,7 +679,7 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : 2) void paged_attn_tile_kernel
         where = (uint64_t)(page < 0 ? 0 : page) * (uint64_t)(P.n_kv * P.block) + (uint64_t)head_off;
         ok = __ballot(page >= 0);
     };
-    uint32_t code[SETS][G], scale[SETS][2 * G];  // a step as it is stored: keys in set 0, values in the last
+    uint32_t kr[G], vr[G], kd[G / 2], vd[2 * G];  // a step as it is stored: codes and scales of keys and values
     bool here = false;
     const int kt = lane >> 2, kc = lane & 3, quad = lane >> 4, vc = lane & 15;
     auto load = [&](int s) __attribute__((always_inline)) {
@@ -685,22 +687,10 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : 2) void paged_attn_tile_kernel
         const uint64_t at = lane_u64(where, l);
         const uint32_t off = (uint32_t)__builtin_amdgcn_readlane(off_tok, l), sc = (uint32_t)P.ps * (16 * G);
         here = (ok >> l) & 1;
-        if (W == 4) {
-            __builtin_memcpy(code[0], P.k + at + (uint32_t)((off + kt) * (16 * G) + kc * (4 * G)), 4 * G);
-            __builtin_memcpy(scale[0], P.k + at + sc + (off + kt) * (2 * G), 2 * G);
-            __builtin_memcpy(code[SETS - 1], P.v + at + (uint32_t)(off * (16 * G) + quad * (64 * G) + vc * (4 * G)),
-                             4 * G);
-            __builtin_memcpy(scale[SETS - 1], P.v + at + sc + (off + 4 * quad) * (2 * G), 8 * G);
-        } else {
-            const uint8_t *pool = wave < 4 ? P.k : P.v;
-            const uint32_t c = wave < 4 ? (uint32_t)(kt * (16 * G) + kc * (4 * G)) : (uint32_t)(quad * (64 * G) + vc * (4 * G));
-            const uint32_t d = wave < 4 ? (uint32_t)(kt * (2 * G)) : (uint32_t)(4 * quad * (2 * G));
-            __builtin_memcpy(code[0], pool + at + off * (16 * G) + c, 4 * G);
-            if (wave < 4)
-                __builtin_memcpy(scale[0], pool + at + sc + off * (2 * G) + d, 2 * G);
-            else
-                __builtin_memcpy(scale[0], pool + at + sc + off * (2 * G) + d, 8 * G);
-        }
+        __builtin_memcpy(kr, P.k + at + (uint32_t)((off + kt) * (16 * G) + kc * (4 * G)), 4 * G);
+        __builtin_memcpy(kd, P.k + at + sc + (off + kt) * (2 * G), 2 * G);
+        __builtin_memcpy(vr, P.v + at + (uint32_t)(off * (16 * G) + quad * (64 * G) + vc * (4 * G)), 4 * G);
+        __builtin_memcpy(vd, P.v + at + sc + (off + 4 * quad) * (2 * G), 8 * G);
     };
     if (s_lo < s_hi) {
         look(s_lo);
@@ -770,39 +760,37 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : 2) void paged_attn_tile_kernel
     // Before the barrier in front of a step's unpacking: the values' scales that no
     // row sees become 0, the largest of the others and the page's presence are told.
     auto tell = [&](int s) __attribute__((always_inline)) {
-        uint32_t(&vd)[2 * G] = scale[SETS - 1];
-        uint32_t most = 0;
-        const int t0 = rg.first + s * 64 + 16 * w4;
-        if (do_v) {
-            if (!(t0 >= rg.lo && t0 + 16 <= rg.hi && here)) {
+        const int t0 = rg.first + s * 64 + 16 * wave;
+        if (!(t0 >= rg.lo && t0 + 16 <= rg.hi && here)) {
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int t = t0 + 4 * quad + r;
-                    const bool out = t < rg.lo || t >= rg.hi || !here;
+            for (int r = 0; r < 4; r++) {
+                const int t = t0 + 4 * quad + r;
+                const bool out = t < rg.lo || t >= rg.hi || !here;
 #pragma unroll
-                    for (int g = 0; g < G; g++) {
-                        const int e = r * G + g;
-                        vd[e >> 1] &= out ? (e & 1 ? 0x0000FFFFu : 0xFFFF0000u) : 0xFFFFFFFFu;
-                    }
+                for (int g = 0; g < G; g++) {
+                    const int e = r * G + g;
+                    vd[e >> 1] &= out ? (e & 1 ? 0x0000FFFFu : 0xFFFF0000u) : 0xFFFFFFFFu;
                 }
             }
-            typedef uint16_t u16x2v __attribute__((ext_vector_type(2)));
-            u16x2v top = {0, 0};
-#pragma unroll
-            for (int j = 0; j < 2 * G; j++) {
-                const uint32_t a = vd[j] & 0x7FFF7FFFu;
-                top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2v, a));
-            }
-            most = top[0] > top[1] ? top[0] : top[1];
-            if (__ballot(most > limit)) {
-                for (int o = 32; o > 0; o >>= 1) {
-                    const uint32_t y = (uint32_t)__shfl_xor((int)most, o, 64);
-                    most = most > y ? most : y;
-                }
-            }
-            if (lane == 0) s_most[s & 1][w4] = most;
         }
-        if (do_k && lane == 0) s_page[s & 1][w4] = here ? 1u << w4 : 0u;
+        typedef uint16_t u16x2v __attribute__((ext_vector_type(2)));
+        u16x2v top = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 2 * G; j++) {
+            const uint32_t a = vd[j] & 0x7FFF7FFFu;
+            top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2v, a));
+        }
+        uint32_t most = top[0] > top[1] ? top[0] : top[1];
+        if (__ballot(most > limit)) {
+            for (int o = 32; o > 0; o >>= 1) {
+                const uint32_t y = (uint32_t)__shfl_xor((int)most, o, 64);
+                most = most > y ? most : y;
+            }
+        }
+        if (lane == 0) {
+            s_most[s & 1][wave] = most;
+            s_page[s & 1][wave] = here ? 1u << wave : 0u;
+        }
     };
     // Behind it: E and the pages of the step.  True where some scales are NaN or
     // infinite.
@@ -828,14 +816,14 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : 2) void paged_attn_tile_kernel
         return bad;
     };
     auto unpack = [&](int s, int b, int e_new, bool bad) __attribute__((always_inline)) {
-        if (do_k) {  // token kt's channels 32 g + 8 kc ..
-            const int t = 16 * w4 + kt;
+        {  // token kt's channels 32 g + 8 kc ..
+            const int t = 16 * wave + kt;
 #pragma unroll
             for (int g = 0; g < G; g++) {
-                const _Float16 d = paged_h2(scale[0][g >> 1])[g & 1];
+                const _Float16 d = paged_h2(kd[g >> 1])[g & 1];
                 const half2v d2 = {d, d};
                 // in the order 0 4 1 5 2 6 3 7 of each eight channels, as the queries
-                const u32x4v c = __builtin_bit_cast(u32x4v, magic.k8(code[0][g]));
+                const u32x4v c = __builtin_bit_cast(u32x4v, magic.k8(kr[g]));
                 u32x4v hi, lo;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
@@ -853,9 +841,7 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : 2) void paged_attn_tile_kernel
                 if (F32) s_k[b][N - 1][k_at(t, 4 * g + kc)] = __builtin_bit_cast(half8v, lo);
             }
         }
-        if (do_v) {  // quad's four tokens, channels 32 g + vc and 32 g + 16 + vc
-            uint32_t(&vd)[2 * G] = scale[SETS - 1];
-            uint32_t(&vr)[G] = code[SETS - 1];
+        {  // quad's four tokens, channels 32 g + vc and 32 g + 16 + vc
             if (bad) {
                 // such groups become 0 here and NaN to the rows that see them
 #pragma unroll
@@ -864,7 +850,7 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : 2) void paged_attn_tile_kernel
                     for (int g = 0; g < G; g++) {
                         const int e = r * G + g;
                         const bool is = ((vd[e >> 1] >> (16 * (e & 1))) & 0x7FFFu) >= 0x7C00u;
-                        if (vc == 0) s_bad[s & 1][16 * w4 + 4 * quad + r][g] = is;
+                        if (vc == 0) s_bad[s & 1][16 * wave + 4 * quad + r][g] = is;
                         vd[e >> 1] &= is ? (e & 1 ? 0x0000FFFFu : 0xFFFF0000u) : 0xFFFFFFFFu;
                     }
             }
@@ -874,7 +860,7 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : 2) void paged_attn_tile_kernel
             uint32_t dv[2 * G];
 #pragma unroll
             for (int j = 0; j < 2 * G; j++) dv[j] = __builtin_bit_cast(uint32_t, paged_h2(vd[j]) * up1 * up2);
-            const int piece = 2 * w4 + (quad & 1);
+            const int piece = 2 * wave + (quad & 1);
 #pragma unroll
             for (int g = 0; g < G; g++) {
                 uint32_t hi[2][2], lo[2][2];

@@ -4476,10 +4476,10 @@ struct PagedDevice {
 static bool paged_quads(uint32_t n_rows) { return n_rows >= 2048; }
 
 // How a call's attention is cut.  Sessions of few rows (R of tokens x query heads of
-// a kv head) are a row tile each; the others are tiles of 32 rows per wave.
+// a kv head) are a row tile each; the others are tiles of 128 rows.
 struct PagedPlan {
     int R = 0, W = 0, short_q = 0, splits = 1, steps = 0;  // row tiles, short_q = 0: none
-    int waves = 0, tok_tile = 0, tile_splits = 1, tile_steps = 0;  // larger tiles, tok_tile = 0: none
+    int tok_tile = 0, tile_splits = 1, tile_steps = 0;     // 128-row tiles, tok_tile = 0: none
     int64_t tiles = 0, heads_y = 0;
 };
 static PagedPlan paged_plan(const PagedDev &P, uint32_t n_heads, uint32_t max_q, uint32_t max_kv, uint32_t window) {
@@ -4516,18 +4516,13 @@ static PagedPlan paged_plan(const PagedDev &P, uint32_t n_heads, uint32_t max_q,
         p.steps = (int)per;
     }
     if (tiles) {
-        // Two workgroups of 4 waves per CU overlap each other's products and
-        // exponentials; one of 8 unpacks keys and values half as often.  64-channel
-        // heads gain by the latter (a chunk of 400 tokens, 64 heads: 97 us a step,
-        // 100), 128-channel ones by the former (512 tokens: 33 us, 41); wider ones
-        // fill the registers of 4.
-        p.waves = P.hd > 64 || P.vd > 64 || (int64_t)max_q * chunk <= 128 ? 4 : 8;
-        p.tok_tile = 32 * p.waves / chunk;
+        p.tok_tile = 128 / chunk;
         p.tiles = P.n_tokens / p.tok_tile + (int64_t)P.n_seqs;
-        // splits of 4 steps or more, as long as eight waves per CU take to share all steps:
-        // the shorter last ones fill the gaps
+        // splits of 4 steps or more, as long as the workgroups that the card holds take to
+        // share all steps; the shorter last ones fill the gaps (a chunk of 400 tokens
+        // behind 3100, 64 heads of 64 channels: 84 us a step with all 768, 98 with 512)
         const int64_t steps = steps_of(p.tok_tile), items = (P.n_tokens + p.tok_tile - 1) / p.tok_tile * p.heads_y;
-        const int64_t slots = 256 * 8 / p.waves;
+        const int64_t slots = 256 * paged_tiles_per_cu(paged_groups(P.hd, P.vd));
         int64_t per = (steps * items + slots - 1) / slots;
         if (per < 4) per = 4;
         if ((steps + per - 1) / per > 256) per = (steps + 255) / 256;
@@ -4569,10 +4564,7 @@ static void paged_attn_launch(const PagedDev &P, PagedAttn A, const PagedPlan &p
     if (p.tok_tile) {
         tiles_of(p.tok_tile, p.tile_splits, p.tile_steps, 1 << 16);
         const dim3 grid((unsigned)(p.tiles * p.heads_y), (unsigned)p.tile_splits);
-        if (p.waves == 4)
-            paged_attn_tile_kernel<G, F32, 4><<<grid, 256, 0, s>>>(P, A);
-        else if constexpr (G != 8)
-            paged_attn_tile_kernel<G, F32, 8><<<grid, 512, 0, s>>>(P, A);
+        paged_attn_tile_kernel<G, F32><<<grid, 256, 0, s>>>(P, A);
         if (p.tile_splits > 1)
             paged_attn_join_tiles_kernel<G, F32>
                 <<<(unsigned)(((int64_t)P.n_tokens * ((A.n_heads + 3) / 4) + 3) / 4), 256, 0, s>>>(P, A);
