@@ -913,12 +913,12 @@ __global__ __launch_bounds__(256, paged_tiles_per_cu(G)) void paged_attn_tile_ke
     for (int s = s_lo; s < s_hi; s++) {
         const int t0 = rg.first + s * 64, b = s & (NB - 1);
         const bool more = s + 1 < s_hi;
-        if (more) tell(s + 1);
+        if (NB == 2 && more) tell(s + 1);
         __syncthreads();  // step s is in LDS; nobody reads step s - 1 any more
         pages = pages_next;
         const bool full = t0 >= full_lo && t0 + 64 <= full_hi && pages == 15;
         e_next = E;
-        if (more) bad_next = decide(s + 1, &e_next);
+        if (NB == 2 && more) bad_next = decide(s + 1, &e_next);
 
         // scores of 64 tokens: [32-token tile][16]
         f32x16v sc[2];
@@ -1006,7 +1006,9 @@ __global__ __launch_bounds__(256, paged_tiles_per_cu(G)) void paged_attn_tile_ke
             }
         }
         if (NB == 1 && more) {
+            tell(s + 1);
             __syncthreads();
+            bad_next = decide(s + 1, &e_next);
             unpack(s + 1, 0, e_next, bad_next);
             load_next(s + 2);
         }
