@@ -395,7 +395,7 @@ typedef struct {
     const float *sinks;         /* [n_heads] or null */
     uintptr_t sinks_len;
     float scale;
-    uint32_t window;            /* row at p sees (p - window, p]; 0 = all of [0, p] */
+    uint32_t window;            /* row at p sees (p - window, p], at most 2^30; 0 = all of [0, p] */
     void *workspace;            /* rusty_hip_paged_attention_workspace bytes, 16-byte aligned; may be null if that is 0 */
     uintptr_t workspace_len;
 } RustyPagedAttention;
@@ -420,9 +420,11 @@ uint64_t rusty_hip_paged_attention_workspace(const RustyPagedKv *kv, const Rusty
                                              uint32_t n_heads);
 /* Softmax attention of the rows' queries over their session's cached positions,
  * causal from each row's own position, with sliding window and per-head sinks
- * (as rusty_hip_attention).  A row whose masks leave nothing is 0.  Sums,
- * maxima and scores are f32; for f32 rows every product keeps at least 16 bits
- * of its factors, for bf16 rows p is rounded to bf16. */
+ * (as rusty_hip_attention).  A row whose masks leave nothing is 0.  Sums, maxima
+ * and scores are f32; the factors of the products on the matrix cores keep 22
+ * bits for f32 rows and 11 for bf16 rows.  What a row does not see may hold
+ * anything, NaN and infinities among it; a group of values whose scale is NaN
+ * makes that group's channels NaN in the rows that see it. */
 int rusty_hip_paged_attention(const RustyPagedKv *kv, const RustyPagedBatch *batch, const RustyPagedAttention *rows,
                               void *stream);
 

@@ -165,9 +165,10 @@ __device__ __forceinline__ uint64_t shfl_u64(uint64_t v, int l) {
 // for f32 rows: 22 bits), where E, the same for the wave, keeps the largest |d| seen
 // near 2^14, so p d leaves the normal halves only 2^28 below the largest.
 //
-// The W = 1 or 4 waves of a workgroup take a tile's steps in turn and join their
-// results.  Neighbouring workgroups are the kv heads of one tile, so the sessions
-// spread over the 8 XCDs (a session each made the XCD with the longest ones last).
+// The W = 4 waves of a workgroup take a tile's steps in turn and join their results;
+// W = 1 is for many short sessions.  Neighbouring workgroups are the kv heads of one
+// tile, so the sessions spread over the 8 XCDs (a session each made the XCD with the
+// longest ones last).
 template <int G, int R, bool F32, int W>
 __global__ __launch_bounds__(64 * W, G == 8 ? 1 : G == 4 ? (R == 4 && !F32 ? 3 : 2) : R == 4 ? 4 : 3) void paged_attn_rows_kernel(PagedDev P, PagedAttn A) {
     constexpr int NT = 16 / R;  // token tiles per score result
@@ -509,32 +510,16 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : G == 4 ? (R == 4 && !F32 ? 3 :
         load_v((more ? k + 1 : k) & 15);
     }
 
-    // a row's lanes hold parts of its sum
     if (NT >= 4) l += paged_dpp<0x124>(l);
     if (NT >= 2) l += paged_dpp<0x128>(l);
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
-    if (W == 1) {  // the wave's lanes hold whole results: four channels of a row each
+    if (W == 1) {  // one split, and the lanes hold whole results: four channels of a row each
         if (col >= R || !on) return;
         const int hd = kvh * A.kv_mul + h0 + my_head;
         const int64_t token = row0 + my_tok;
         const bool none = m == -__builtin_inff();
         const float one = ldexpf(1.0f, -(int)E);
-        if (A.n_splits > 1) {
-            const int64_t to = ((int64_t)split * P.n_tokens + token) * A.n_heads + hd;
-            if (quad == 0) {
-                A.ml[to * 2] = m;
-                A.ml[to * 2 + 1] = l * one;
-            }
-#pragma unroll
-            for (int g = 0; g < G; g++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const float y[4] = {acc[g][h][0] * one, acc[g][h][1] * one, acc[g][h][2] * one, acc[g][h][3] * one};
-                    if (!none) row_store4(A.part + to * DV + 32 * g + 16 * h + 4 * quad, y);
-                }
-            return;
-        }
         float f = none ? 0.0f : 1.0f / l;
         if (A.sinks && !none) {
             const float sink = A.sinks[hd] * 1.44269504f, top = fmaxf(m, sink), a = __builtin_amdgcn_exp2f(m - top);
@@ -1027,6 +1012,7 @@ __global__ __launch_bounds__(256, paged_tiles_per_cu(G)) void paged_attn_tile_ke
     const float unit = ldexpf(1.0f, -E - 6);
     // the arguments used from here on are read here: kept through the loop, they
     // pushed others out of the scalar registers (25 lane reads per step)
+    static_assert(sizeof(PagedDev) % alignof(PagedAttn) == 0, "the second argument follows the first");
     typedef __attribute__((address_space(4))) const uint8_t kernarg_t;
     kernarg_t *args = (kernarg_t *)__builtin_amdgcn_kernarg_segment_ptr() + sizeof(PagedDev);
     asm volatile("" : "+s"(args));

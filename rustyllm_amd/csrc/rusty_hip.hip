@@ -4505,12 +4505,9 @@ static PagedPlan paged_plan(const PagedDev &P, uint32_t n_heads, uint32_t max_q,
         // three workgroups per CU: 48 ragged sessions of up to 8192 take 76 us with 64
         // steps, 80 with 16; one of 131072 takes 36 and 43.
         p.W = items >= 2048 && steps <= 16 ? 1 : 4;
-        int64_t per = 16;
-        if (p.W == 4) {
-            per = (steps * items + 767) / 768;
-            per = per < 4 ? 4 : per > 64 ? 64 : per;
-        }
-        if (steps <= per + per / 2) per = steps;
+        int64_t per = (steps * items + 767) / 768;
+        per = per < 4 ? 4 : per > 64 ? 64 : per;
+        if (p.W == 1 || steps <= per + per / 2) per = steps;
         if ((steps + per - 1) / per > 256) per = (steps + 255) / 256;
         p.splits = (int)((steps + per - 1) / per);
         p.steps = (int)per;
@@ -4714,12 +4711,17 @@ int rusty_hip_paged_attention(const RustyPagedKv *kv, const RustyPagedBatch *bat
     if (!rows_ok(rows->q, rows->q_len, n, rows->q_stride, (int64_t)rows->n_heads * P.hd, item) ||
         !rows_ok(rows->out, rows->out_len, n, rows->out_stride, (int64_t)rows->n_heads * P.vd, item) ||
         (rows->sinks && ((uintptr_t)rows->sinks % 4 || rows->sinks_len < (uint64_t)rows->n_heads * 4)) ||
-        rows->window > 0x7FFFFFFFu || !(rows->scale == rows->scale))
+        rows->window > (1u << 30) || !(rows->scale == rows->scale))
         return 0;
     PagedDevice dev((hipStream_t)stream);
     if (!dev.ok) return 0;
-    const PagedPlan p = paged_plan(P, rows->n_heads, batch->max_q_len, batch->max_kv_len, rows->window);
-    const uint64_t need = paged_workspace(P, p, rows->n_heads);
+    PagedPlan p = paged_plan(P, rows->n_heads, batch->max_q_len, batch->max_kv_len, rows->window);
+    uint64_t need = paged_workspace(P, p, rows->n_heads);
+    if (rows->window && need > rows->workspace_len) {
+        // the size was told without the window, whose shorter splits may round to more of them
+        p = paged_plan(P, rows->n_heads, batch->max_q_len, batch->max_kv_len, 0);
+        need = paged_workspace(P, p, rows->n_heads);
+    }
     if (need && (!rows->workspace || rows->workspace_len < need || (uintptr_t)rows->workspace % 16)) return 0;
     if (p.tiles * p.heads_y > (0x7FFFFFFF >> 8) || P.n_seqs * p.heads_y > (0x7FFFFFFF >> 8) ||
         (int64_t)P.n_seqs * p.short_q * rows->n_heads > (0x7FFFFFFF >> 8) || (int64_t)n * rows->n_heads > 0x7FFFFFFF) return 0;

@@ -208,6 +208,109 @@ def test_masked_nan_and_infinities_stay_out(hip, dtype):
     assert (np.abs(got - ref) <= tol)[rows].all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,n_kv,hd", [(16, 16, 64), (80, 16, 64), (128, 8, 64), (48, 16, 128), (8, 8, 256)])
+def test_many_short_sessions(hip, heads, n_kv, hd, dtype):
+    """Enough (session, kv head) pairs that each is one wave's: 1, 5, 16 and 3 query
+    heads per kv head, with a window that cuts and sinks."""
+    n = -(-2048 // n_kv)
+    rng = np.random.default_rng(heads)
+    lens = [int(x) for x in rng.integers(1, 19, n)]
+    lens[:5] = [0, 40, 1, 70, 16]
+    s = Setup(hip, heads, n_kv, hd, [(a, 1) for a in lens], dtype=dtype, seed=heads).fill().upload()
+    q = s.round(1.5 * s.randn(s.n, heads, hd))
+    assert s.workspace(s.n) is None  # nothing is split
+    s.attend(q, 9, 2 * s.randn(heads))
+
+
+def test_heads_that_do_not_share_evenly_are_refused(hip):
+    """24 query heads of 16 kv heads, many sessions: no workspace and no call."""
+    import torch
+    s = Setup(hip, 24, 16, 128, [(16, 1)] * 128, seed=24).fill().upload()
+    out = torch.full((s.n, 24, 128), 7.0, device=DEV)
+    assert hip.paged_attention_workspace(s.cache, s.batch, s.n, 24) == 0
+    assert not hip.paged_attention_dev(s.cache, s.batch, _t(s.randn(s.n, 24, 128)), out, 0.1, None, window=9)
+    assert bool((out == 7.0).all())
+
+
+@pytest.mark.parametrize("sessions,most", [([(4928, 1), (70, 1), (4700, 1), (9, 1), (700, 1)], 4928),
+                                           ([(3520, 100)], 3520)])
+def test_windows_split_finer_than_the_whole_row(hip, sessions, most):
+    """A window a little shorter than the context: its splits round to more than those
+    of the whole row, for which the workspace is told."""
+    import torch
+    s = Setup(hip, 64, 8, 64, sessions, dtype="bf16", seed=most).fill().upload()
+    q = s.round(s.randn(s.n, 64, 64))
+    tq, ws = _t(q, torch.bfloat16), s.workspace(s.n)
+    out = torch.empty_like(tq)
+    for window in range(32, most, 32):
+        assert hip.paged_attention_dev(s.cache, s.batch, tq, out, 0.125, ws, window=window), window
+    for window in (most * 8 // 9, most - 40):
+        s.attend(q, window)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,n_kv,hd,window", [(8, 1, 64, 0), (4, 2, 128, 100), (5, 1, 128, 0), (2, 1, 256, 0),
+                                                  (40, 2, 64, 0)])
+def test_long_chunks(hip, heads, n_kv, hd, window, dtype):
+    """Several tiles of one chunk, split over its cached rows, next to sessions of
+    single tokens and a chunk of another length."""
+    s = Setup(hip, heads, n_kv, hd, [(300, 1), (460, 71), (5, 1), (333, 33)], ps=32, dtype=dtype, seed=heads + hd).fill()
+    s.upload()
+    s.attend(s.round(1.5 * s.randn(s.n, heads, hd)), window, 2 * s.randn(heads) if window else None)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_scales_that_grow_and_shrink_along_the_row(hip, rows, dtype):
+    """Values of 1e-4 at first, then 1, 300 and 1e-3: the common exponent follows the
+    largest and nothing of the others is lost that matters."""
+    s = Setup(hip, 8, 2, 64, [(400, rows)], dtype=dtype, seed=91)
+    p = s.pool
+    for t in range(400):
+        size = np.float32([1e-4, 1.0, 300.0, 1e-3][t // 100])
+        p.store("k", s.table[0, t // p.ps], t % p.ps, s.randn(2, 64))
+        p.store("v", s.table[0, t // p.ps], t % p.ps, s.randn(2, 64) * size)
+    s.upload()
+    q = s.round(s.randn(rows, 8, 64))
+    s.attend(q)
+    s.kv_lens[0] = 110  # rows that see the small values and few of the next
+    s.upload()
+    s.attend(q)
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+def test_nan_group_is_nan_where_it_is_seen(hip, rows):
+    """One NaN scale of a value's second group: those 32 channels of the rows at and
+    behind it, and nothing else."""
+    import torch
+    s = Setup(hip, 8, 2, 64, [(130, rows), (70, 1)], seed=92).fill()
+    p = s.pool
+    t = 130 - rows // 2 - 1  # inside the chunk
+    page, off = s.table[0, t // p.ps], t % p.ps
+    q = s.randn(s.n, 8, 64)
+    ref, spread, size = R.attention(p, s.table, s.kv_lens, s.q_starts, q, 0.125)
+    at = p._at(page, 1) + p.ps * 16 * p.G + (off * p.G + 1) * 2
+    p.v[at:at + 2].view(np.uint16)[:] = 0x7E00
+    s.upload()
+    out = torch.zeros(s.n, 8, 64, device=DEV)
+    assert hip.paged_attention_dev(s.cache, s.batch, _t(q), out, 0.125, s.workspace(s.n))
+    got = out.cpu().numpy()
+    want = np.zeros(got.shape, bool)
+    sees = np.arange(s.n) >= rows - (130 - t)
+    sees[rows:] = False
+    want[sees, 4:, 32:] = True  # heads 4.. share kv head 1
+    assert np.array_equal(np.isnan(got), want)
+    assert (np.abs(got - ref) <= R.tolerance(ref, spread, size, "f32"))[~want].all()
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_negative_and_zero_scale(hip, rows, scale):
+    s = Setup(hip, 8, 2, 64, [(150, rows), (90, 1)], seed=93).fill().upload()
+    s.attend(s.randn(s.n, 8, 64), scale=scale)
+
+
 def test_rows_behind_the_last_session_are_left(hip):
     import torch
     s = Setup(hip, 4, 2, 64, [(20, 1), (300, 2)], seed=15).fill().upload()
@@ -331,12 +434,11 @@ def test_append_leaves_out_what_has_no_place(hip):
 
 
 def test_append_far_positions_and_large_pools(hip):
-    """A position near the end of a 128 K context, in a pool whose bytes pass 2^31
-    (2^32 for K and V together)."""
+    """A position near the end of a 128 K context, in pages whose bytes pass 2^32."""
     import torch
-    n_pages, ps, n_kv, hd = 4000, 1024, 8, 128
+    n_pages, ps, n_kv, hd = 8000, 1024, 8, 128
     size = hip.paged_kv_bytes(n_pages, ps, n_kv, hd)
-    assert size > 2 ** 31
+    assert size > 2 ** 32
     k_dev, v_dev = (torch.zeros(size, dtype=torch.uint8, device=DEV) for _ in range(2))
     cache = hip.PagedKv(k_dev, v_dev, n_pages, ps, n_kv, hd)
     table = np.full((2, 128), -1, np.int32)
@@ -456,6 +558,48 @@ def test_captured_and_replayed(hip):
         step()
         torch.cuda.synchronize()
         assert torch.equal(out, got) and torch.equal(s.k_dev, pools[0]) and torch.equal(s.v_dev, pools[1])
+
+
+def test_a_captured_chunk(hip):
+    """A prompt's chunk and decoding sessions in one graph, replayed over other
+    queries and lengths."""
+    import torch
+    s = Setup(hip, 8, 2, 64, [(300, 60), (90, 1), (400, 1)], dtype="bf16", seed=94).fill().upload()
+    q = _t(s.randn(s.n, 8, 64), torch.bfloat16)
+    out, ws = torch.empty_like(q), s.workspace(s.n)
+    call = lambda: hip.paged_attention_dev(s.cache, s.batch, q, out, 0.125, ws)  # noqa: E731
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        assert call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert call()
+    start = torch.tensor([250, 40, 350], dtype=torch.int32, device=DEV)
+    for i in range(3):
+        s.t_lens.copy_(start + 17 * i)
+        q.copy_(torch.randn_like(q))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        out.fill_(7.0)
+        assert call()
+        torch.cuda.synchronize()
+        assert torch.equal(out, got)
+
+
+def test_the_current_device_and_stream_are_the_callers(hip):
+    """A call on a stream given by handle, and torch's current device as it was."""
+    import torch
+    s = Setup(hip, 4, 2, 64, [(90, 1), (20, 2)], seed=95).fill().upload()
+    q, st = s.randn(3, 4, 64), torch.cuda.Stream()
+    tq, out, ws = _t(q), torch.zeros(3, 4, 64, device=DEV), s.workspace(3)
+    torch.cuda.synchronize()
+    assert hip.paged_attention_dev(s.cache, s.batch, tq, out, 0.125, ws, stream=st.cuda_stream)
+    st.synchronize()
+    assert torch.cuda.current_device() == 0
+    ref, spread, size = R.attention(s.pool, s.table, s.kv_lens, s.q_starts, q, 0.125)
+    assert (np.abs(out.cpu().numpy() - ref) <= R.tolerance(ref, spread, size, "f32")).all()
 
 
 def test_two_streams_at_once(hip):
