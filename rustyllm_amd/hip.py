@@ -7,7 +7,9 @@ False when the caller must run its CPU kernel (src/metal.rs:716-720).
 for the reference (src/metal.rs:586-631).
 
 Importing this module loads the library and raises if it is missing: there is
-no silent fallback inside the product path.
+no silent fallback inside the product path.  A program that also uses torch
+imports torch first: the library then shares the HIP runtime that torch brings.
+The other way round there are two in the process, and torch finds no GPU.
 """
 from __future__ import annotations
 
@@ -730,12 +732,23 @@ def _dev_bytes(t, what, dtype):
     return t.data_ptr(), t.nbytes
 
 
+def _one_runtime():
+    """Raises where torch and the library run on two HIP runtimes, for which a
+    stream or a tensor of the other is nothing."""
+    with open("/proc/self/maps") as f:
+        found = {line.split()[-1] for line in f if "libamdhip64" in line}
+    if len(found) > 1:
+        raise RuntimeError("two HIP runtimes are loaded (" + ", ".join(sorted(found)) +
+                           "): import torch before rustyllm_amd.hip")
+
+
 class PagedKv:
     """One layer's pool of cache pages (RustyPagedKv) over two uint8 device
     tensors of paged_kv_bytes each.  The tensors stay the caller's."""
 
     def __init__(self, k_pages, v_pages, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
                  value_dim: int | None = None):
+        _one_runtime()
         self.n_kv_heads, self.head_dim, self.value_dim = n_kv_heads, head_dim, value_dim or head_dim
         k, k_len = _dev_bytes(k_pages, "k_pages", "uint8")
         v, v_len = _dev_bytes(v_pages, "v_pages", "uint8")

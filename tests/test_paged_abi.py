@@ -1,9 +1,13 @@
 """The paged cache's host side without a GPU: sizes, structs and refusals, and
 the plain form's own layout."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
+import torch  # noqa: F401  before the library, which then shares torch's HIP runtime
 
 from rustyllm_amd import hip
 from tests import paged_ref as R
@@ -160,3 +164,18 @@ def test_attention_of_the_plain_form_is_softmax():
     for r in range(2):
         w = np.exp(0.3 * k[:34 + r] @ q[r].T.astype(np.float64))
         assert np.allclose(out[r], (w / w.sum(0)).T @ v[:34 + r], rtol=1e-12)
+
+
+@pytest.mark.parametrize("first,second,refused", [("torch", "rustyllm_amd.hip", False),
+                                                  ("rustyllm_amd.hip", "torch", True)])
+def test_two_hip_runtimes_are_refused(first, second, refused):
+    """torch brings a HIP runtime of its own: loaded behind the library there are two
+    in the process, and a stream or tensor of one means nothing to the other."""
+    code = (f"import {first}, {second}\nimport torch\nfrom rustyllm_amd import hip\n"
+            "t = torch.zeros(hip.paged_kv_bytes(1, 16, 1, 64), dtype=torch.uint8)\n"
+            "try:\n    hip.PagedKv(t, t, 1, 16, 1, 64)\n"
+            "except Exception as e:\n    print(type(e).__name__)\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    # a CPU tensor is a ValueError, once the runtimes are found to be one
+    assert run.stdout.strip() == ("RuntimeError" if refused else "ValueError"), run.stderr
