@@ -357,10 +357,10 @@ typedef struct {
     uint32_t max_kv_len;        /* about the longest session; sizes the work's split, any value is correct */
 } RustyPagedBatch;
 
-/* Row buffers: n_rows rows each, the last session's end or more; row r of x starts at x + r * x_stride elements (float, or bf16
- * with dtype = 1); rows are [heads][dim] without gaps.  Bases are aligned to
- * four elements, strides are multiples of four.  x_len: bytes from x that the
- * call may touch. */
+/* Row buffers: n_rows rows each, the last session's end or more; row r of x starts
+ * at x + r * x_stride elements (float, or bf16 with dtype = 1); rows are
+ * [heads][dim] without gaps.  Bases are aligned to four elements, strides are
+ * multiples of four.  x_len: bytes from x that the call may touch. */
 typedef struct {
     uint32_t dtype;             /* of all rows: 0 = f32, 1 = bf16 */
     uint32_t n_rows;
@@ -423,8 +423,9 @@ uint64_t rusty_hip_paged_attention_workspace(const RustyPagedKv *kv, const Rusty
  * (as rusty_hip_attention).  A row whose masks leave nothing is 0.  Sums, maxima
  * and scores are f32; the factors of the products on the matrix cores keep 22
  * bits for f32 rows and 11 for bf16 rows.  What a row does not see may hold
- * anything, NaN and infinities among it; a group of values whose scale is NaN
- * makes that group's channels NaN in the rows that see it. */
+ * anything, NaN and infinities among it; a NaN in a query, or in a key that a row
+ * sees, makes that row of the head NaN, and a group of values whose scale is NaN
+ * that group's channels.  out may not overlap q. */
 int rusty_hip_paged_attention(const RustyPagedKv *kv, const RustyPagedBatch *batch, const RustyPagedAttention *rows,
                               void *stream);
 

@@ -514,6 +514,9 @@ __global__ __launch_bounds__(64 * W, G == 8 ? 1 : G == 4 ? (R == 4 && !F32 ? 3 :
     if (NT >= 2) l += paged_dpp<0x128>(l);
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
+    // scores of NaN pass the maximum by, also where there is no other: with +inf the row
+    // is no empty one, and its weight is NaN in every join
+    if (l != l) m = __builtin_inff();
     if (W == 1) {  // one split, and the lanes hold whole results: four channels of a row each
         if (col >= R || !on) return;
         const int hd = kvh * A.kv_mul + h0 + my_head;
@@ -1008,6 +1011,7 @@ __global__ __launch_bounds__(256, paged_tiles_per_cu(G)) void paged_attn_tile_ke
 
     l += __shfl_xor(l, 32, 64);
     l *= 1.0f / 64.0f;
+    if (l != l) m = __builtin_inff();  // as in the row tiles
     if (!on) return;
     const float unit = ldexpf(1.0f, -E - 6);
     // the arguments used from here on are read here: kept through the loop, they

@@ -304,6 +304,51 @@ def test_nan_group_is_nan_where_it_is_seen(hip, rows):
     assert (np.abs(got - ref) <= R.tolerance(ref, spread, size, "f32"))[~want].all()
 
 
+NAN_SESSIONS = {  # kind: sessions, head dim, page size, heads
+    "single": ([(1, 1), (70, 1), (2, 1)], 64, 16, 8),
+    "split": ([(3000, 1), (1, 1), (900, 1)], 128, 64, 8),
+    "one_wave_each": ([(1 + i % 19, 1) for i in range(1024)], 64, 16, 8),
+    "chunk": ([(40, 40), (1, 1), (700, 60)], 64, 16, 8),
+    "wide_chunk": ([(300, 40)], 128, 16, 8),
+    "many_heads": ([(150, 3), (30, 20)], 64, 16, 40),
+}
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("sinks", [False, True])
+@pytest.mark.parametrize("kind", sorted(NAN_SESSIONS))
+def test_nan_queries_and_seen_nan_keys_give_nan(hip, kind, sinks, dtype):
+    """A NaN query, and a NaN key that a row sees, make all of that row's channels NaN
+    (of the heads concerned), also where no other score is left, and no other row's."""
+    import torch
+    sessions, hd, ps, heads = NAN_SESSIONS[kind]
+    s = Setup(hip, heads, 2, hd, sessions, ps=ps, dtype=dtype, seed=96).fill()
+    q, sk = s.round(s.randn(s.n, heads, hd)), s.randn(heads) if sinks else None
+    scale = np.float32(hd ** -0.5)
+    ref, spread, size = R.attention(s.pool, s.table, s.kv_lens, s.q_starts, q, scale, 0, sk)
+    tol = R.tolerance(ref, spread, size, dtype)
+    want = np.zeros(ref.shape, bool)
+    for row, head in ((0, 1), (s.n - 1, heads - 1), (s.n // 2, 0)):
+        q[row, head, 3] = np.nan
+        want[row, head] = True
+    # the last session's key 0 of kv head 1, and the first session's last one of kv head 0
+    p, mul, last = s.pool, heads // 2, len(sessions) - 1
+    for seq, t, h in ((last, 0, 1), (0, int(s.kv_lens[0]) - 1, 0)):
+        page, off = s.table[seq, t // p.ps], t % p.ps
+        at = p._at(page, h) + p.ps * 16 * p.G + off * p.G * 2
+        p.k[at:at + 2 * p.G].view(np.uint16)[:] = 0x7E00
+        for r in range(s.q_starts[seq], s.q_starts[seq + 1]):
+            if s.kv_lens[seq] - (s.q_starts[seq + 1] - r) >= t:
+                want[r, h * mul:(h + 1) * mul] = True
+    s.upload()
+    out = torch.zeros(s.n, heads, hd, dtype=_dtype(dtype), device=DEV)
+    assert hip.paged_attention_dev(s.cache, s.batch, _t(q, _dtype(dtype)), out, scale, s.workspace(s.n),
+                                   None if sk is None else _t(sk))
+    got = out.float().cpu().numpy()
+    assert np.array_equal(np.isnan(got), want), np.argwhere(np.isnan(got) != want)[:4]
+    assert (np.abs(got - ref) <= tol)[~want].all()
+
+
 @pytest.mark.parametrize("scale", [-0.3, 0.0])
 @pytest.mark.parametrize("rows", [1, 40])
 def test_negative_and_zero_scale(hip, rows, scale):
